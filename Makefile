@@ -5,7 +5,10 @@ HIPCC    ?= /opt/rocm/bin/hipcc
 CC       ?= gcc
 CXX      ?= g++
 ARCH     ?= gfx950
-HIPFLAGS ?= -O3 -std=c++17 -fPIC --offload-arch=$(ARCH) -Iinclude -Wall -Wno-unused-function
+# no packed fp32 instructions: some of their forms are not reliable on this hardware (the host pass warns that it
+# does not know the feature, which is harmless)
+NOPACKED := -Xclang -target-feature -Xclang -packed-fp32-ops
+HIPFLAGS ?= -O3 -std=c++17 -fPIC --offload-arch=$(ARCH) -Iinclude -Wall -Wno-unused-function $(NOPACKED)
 
 LIB      := radx_amd/lib/libradx_hip.so
 ORACLE   := oracle/libradx_oracle.so
@@ -16,9 +19,11 @@ REFSEQ   := harness/reference_sequence
 
 all: $(LIB) $(ORACLE) $(CPUSORT) $(HARNESS) $(SHARDED) $(REFSEQ)
 
-$(LIB): radx_amd/csrc/radx_hip.hip include/radx_hip.h
+ENGINE   := radx_amd/csrc/radx_hip.hip radx_amd/csrc/radx_beam.hip
+
+$(LIB): $(ENGINE) radx_amd/csrc/engine_host.h include/radx_hip.h
 	@mkdir -p radx_amd/lib
-	$(HIPCC) $(HIPFLAGS) -shared -o $@ radx_amd/csrc/radx_hip.hip
+	$(HIPCC) $(HIPFLAGS) -shared -o $@ $(ENGINE)
 
 $(ORACLE): oracle/radx_oracle.c oracle/radx_oracle.h
 	$(CC) -O2 -std=c11 -fPIC -shared -Wall -Wextra -o $@ oracle/radx_oracle.c
@@ -62,17 +67,17 @@ harness/sort_test_asan: harness/sort_test.cpp $(LIB) $(wildcard include/radx/*.h
 	    -Wl,-rpath,'$$ORIGIN/../radx_amd/lib' -Wl,-rpath,/opt/rocm/lib
 
 resources:
-	$(HIPCC) $(HIPFLAGS) -Rpass-analysis=kernel-resource-usage -c -o /dev/null radx_amd/csrc/radx_hip.hip 2>&1 | \
+	for f in $(ENGINE); do $(HIPCC) $(HIPFLAGS) -Rpass-analysis=kernel-resource-usage -c -o /dev/null $$f; done 2>&1 | \
 	    grep -E "Function Name|VGPRs:|SGPRs:|Occupancy|LDS Size|ScratchSize" | grep -v "^$$" || true
 
 # development micro-benchmark: HBM copy ceilings by access width and launch shape
 micro: tools/micro/copy_bench tools/micro/rocprim_sort_bench tools/micro/dispatch_bench
 tools/micro/dispatch_bench: tools/micro/dispatch_bench.hip
-	$(HIPCC) -O3 -w --offload-arch=$(ARCH) -o $@ $<
+	$(HIPCC) -O3 -w --offload-arch=$(ARCH) $(NOPACKED) -o $@ $<
 tools/micro/rocprim_sort_bench: tools/micro/rocprim_sort_bench.hip
-	$(HIPCC) -O3 -w --offload-arch=$(ARCH) -o $@ $<
+	$(HIPCC) -O3 -w --offload-arch=$(ARCH) $(NOPACKED) -o $@ $<
 tools/micro/copy_bench: tools/micro/copy_bench.hip
-	$(HIPCC) -O3 -w --offload-arch=$(ARCH) -o $@ $<
+	$(HIPCC) -O3 -w --offload-arch=$(ARCH) $(NOPACKED) -o $@ $<
 
 clean:
 	rm -f $(LIB) $(ORACLE) $(CPUSORT) $(HARNESS) $(SHARDED) $(REFSEQ) tools/micro/copy_bench tools/micro/rocprim_sort_bench \

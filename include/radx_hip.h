@@ -257,6 +257,109 @@ int radx_hip_indiction(uint32_t* ptrs, void* cache, const void* in, uint64_t n, 
 int radx_hip_permutation(void* in, const void* cache, const uint32_t* ptrs, uint64_t n,
                          size_t elem_bytes, void* stream);
 
+/* ---- beam search ----
+ *
+ * What a decoding loop does beside its model, next to the sort: the choice of the k best continuations (the first k
+ * of a descending float order, ties by index), the move of the survivors' states to their new places (rows moved
+ * by an index, as in radx_hip_permutation), and the sequences out of the recorded choices.  None of it has a
+ * counterpart in the reference.  Every call enqueues its kernels on `stream`, allocates nothing and can be
+ * captured into a graph.
+ */
+#define RADX_HIP_F32 0
+#define RADX_HIP_BF16 1
+#define RADX_HIP_F16 2
+
+#define RADX_HIP_BEAM_MAX_BEAMS 64
+#define RADX_HIP_BEAM_MAX_K 128
+#define RADX_HIP_BEAM_MAX_VOCAB (1u << 24)
+#define RADX_HIP_BEAM_MAX_ROWS 64
+
+typedef struct radx_hip_beam radx_hip_beam;
+
+/* Bytes of device scratch a handle for calls within these limits holds (0: limits out of range). */
+size_t radx_hip_beam_scratch_bytes(uint32_t max_batch, uint32_t max_beams, uint32_t max_vocab, uint32_t max_k);
+
+/*
+ * Create the handle of selections of at most max_batch (1..2^20) items x max_beams (1..64) beams x max_vocab
+ * (1..2^24) tokens, max_k (1..128) places, on HIP device `device`.  It owns the scratch of the call in flight: one
+ * selection may be in flight per handle, also between two captured graphs.
+ */
+int radx_hip_beam_create(int device, uint32_t max_batch, uint32_t max_beams, uint32_t max_vocab, uint32_t max_k,
+                         radx_hip_beam** out);
+int radx_hip_beam_destroy(radx_hip_beam* h);
+
+/*
+ * The k best continuations of every batch item, best first:
+ *
+ *   score(b, i, v) = cum[b][i] + log softmax(logits[b * beams + i])[v]      (normalize != 0)
+ *   score(b, i, v) = cum[b][i] + logits[b * beams + i][v]                   (normalize == 0: log probabilities given)
+ *
+ * Compared in 64 bits and rounded to the float that scores[] gets; equal scores go to the lower beam, in a beam
+ * to the larger logit, then to the lower token.
+ *   allowed       bit v & 31 of word v >> 5 of a row: token v may be chosen.  The others count as -inf, in the
+ *                 softmax too, whatever their logits hold.  allowed_stride: words between rows, 0 = one mask for all.
+ *   finished      beams that have ended (bytes, 0 or not): such a beam offers end_token at its cum score and
+ *                 nothing else, its logits are not read.  out_finished[b][j] then says whether place j has ended: its
+ *                 parent had, or its token is end_token.  NULL: no beam has, and out_finished must be NULL.
+ *   A beam offers nothing if its cum score is not finite, no allowed logit is above -inf, or an allowed logit is NaN
+ *   or +inf.  Places that are left over get score -inf, parent -1, token -1 (and not finished).
+ * logits: rows of `vocab` elements of the dtype, row_stride elements apart (any alignment of the rows; 0 = all
+ * beams share one row).  cum, finished: [batch][beams]; the outputs: [batch][k], disjoint from the inputs.
+ */
+typedef struct {
+    const void* logits;
+    uint64_t row_stride;
+    const float* cum;
+    const uint32_t* allowed;
+    uint64_t allowed_stride;
+    const uint8_t* finished;
+    float* scores;
+    int32_t* parents;
+    int32_t* tokens;
+    uint8_t* out_finished;
+    uint32_t batch, beams, vocab, k;
+    int32_t dtype;      /* RADX_HIP_F32, RADX_HIP_BF16 or RADX_HIP_F16 */
+    int32_t normalize;
+    int32_t end_token;  /* read when finished is given */
+} radx_hip_beam_select_args;
+int radx_hip_beam_select(radx_hip_beam* h, const radx_hip_beam_select_args* args, void* stream);
+
+/*
+ * The survivors' states to their places: for every state, item b and j < k,
+ *
+ *   dst row b * dst_beams + j = src row b * src_beams + parents[b][j]
+ *
+ * parents[batch][k] on the device, k <= 64; where a parent is < 0 or >= src_beams the row is left as it was.
+ * In place (dst == src, same layout): rows are read and written as if all were read first, a row that stays
+ * is not touched, rows k.. of an item stay.  Otherwise src and dst must not overlap.  The states of a call must
+ * not share bytes with each other.
+ * A row is outer[0] x outer[1] pieces, src_outer[] / dst_outer[] bytes apart, of units x unit_bytes contiguous
+ * bytes each, at any alignment; rows are src_row / dst_row bytes apart.  lengths (device, [batch], or NULL): of the
+ * units of item b only the first lengths[b] move; what lies behind them is neither read nor written.
+ */
+typedef struct {
+    const void* src;
+    void* dst;
+    uint64_t src_row, dst_row;
+    uint64_t src_outer[2], dst_outer[2];
+    uint64_t unit_bytes, units;
+    uint32_t outer[2];
+} radx_hip_beam_state;
+int radx_hip_beam_reorder(const radx_hip_beam_state* states, uint32_t n_states, const int32_t* parents, const int32_t* lengths,
+                          uint32_t batch, uint32_t src_beams, uint32_t dst_beams, uint32_t k, void* stream);
+
+/*
+ * The sequences of the last step's places out of tokens[total_steps][batch][k] and parents[total_steps][batch][k] as
+ * the selections left them: with L = steps[b] (NULL: total_steps; at most total_steps counts),
+ *
+ *   out[b][j][t] = tokens[t][b][p(t)],   p(L - 1) = j,   p(t - 1) = parents[t][b][p(t)]
+ *
+ * where a parent < 0 or >= k stands for the same place.  out[b][j] begins at out + (b * k + j) * out_stride;
+ * elements from L on are left as they were.  k <= 128, total_steps < 2^24.
+ */
+int radx_hip_beam_backtrace(const int32_t* tokens, const int32_t* parents, const int32_t* steps, uint32_t total_steps, uint32_t batch,
+                            uint32_t k, int32_t* out, uint64_t out_stride, void* stream);
+
 /* ---- harness utilities (device side of src/test/sort.cpp's generation and checking) ---- */
 
 /* keys[i] = H(i ^ seed), H = the 32-bit integer hash of src/test/sort.cpp:226-234. */

@@ -10,10 +10,27 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libradx_hip.so")
 
-# Every symbol include/radx_hip.h declares, with its ctypes signature.
 _u32p = ctypes.POINTER(ctypes.c_uint32)
 _u64p = ctypes.POINTER(ctypes.c_uint64)
 _vp = ctypes.c_void_p
+
+
+class BeamSelectArgs(ctypes.Structure):
+    """radx_hip_beam_select_args."""
+    _fields_ = [("logits", _vp), ("row_stride", ctypes.c_uint64), ("cum", _vp), ("allowed", _vp), ("allowed_stride", ctypes.c_uint64),
+                ("finished", _vp), ("scores", _vp), ("parents", _vp), ("tokens", _vp), ("out_finished", _vp),
+                ("batch", ctypes.c_uint32), ("beams", ctypes.c_uint32), ("vocab", ctypes.c_uint32), ("k", ctypes.c_uint32),
+                ("dtype", ctypes.c_int32), ("normalize", ctypes.c_int32), ("end_token", ctypes.c_int32)]
+
+
+class BeamState(ctypes.Structure):
+    """radx_hip_beam_state."""
+    _fields_ = [("src", _vp), ("dst", _vp), ("src_row", ctypes.c_uint64), ("dst_row", ctypes.c_uint64), ("src_outer", ctypes.c_uint64 * 2),
+                ("dst_outer", ctypes.c_uint64 * 2), ("unit_bytes", ctypes.c_uint64), ("units", ctypes.c_uint64),
+                ("outer", ctypes.c_uint32 * 2)]
+
+
+# Every symbol include/radx_hip.h declares, with its ctypes signature.
 SIGNATURES = {
     "radx_hip_version": (ctypes.c_int, []),
     "radx_hip_error_string": (ctypes.c_char_p, []),
@@ -45,6 +62,12 @@ SIGNATURES = {
     "radx_hip_kernel_times": (ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_double), _u64p]),
     "radx_hip_indiction": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_uint64, ctypes.c_size_t, _vp]),
     "radx_hip_permutation": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_uint64, ctypes.c_size_t, _vp]),
+    "radx_hip_beam_scratch_bytes": (ctypes.c_size_t, [ctypes.c_uint32] * 4),
+    "radx_hip_beam_create": (ctypes.c_int, [ctypes.c_int] + [ctypes.c_uint32] * 4 + [ctypes.POINTER(_vp)]),
+    "radx_hip_beam_destroy": (ctypes.c_int, [_vp]),
+    "radx_hip_beam_select": (ctypes.c_int, [_vp, ctypes.POINTER(BeamSelectArgs), _vp]),
+    "radx_hip_beam_reorder": (ctypes.c_int, [ctypes.POINTER(BeamState), ctypes.c_uint32, _vp, _vp] + [ctypes.c_uint32] * 4 + [_vp]),
+    "radx_hip_beam_backtrace": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, _vp, ctypes.c_uint64, _vp]),
     "radx_hip_generate_u32": (ctypes.c_int, [_vp, ctypes.c_uint64, ctypes.c_uint32, _vp]),
     "radx_hip_generate_u64": (ctypes.c_int, [_vp, _vp, ctypes.c_uint64, ctypes.c_uint32, _vp]),
     "radx_hip_check_sorted": (ctypes.c_int, [_vp, _vp, ctypes.c_uint64, ctypes.c_int, _u64p, _vp]),

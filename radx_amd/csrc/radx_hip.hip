@@ -51,7 +51,10 @@
 #include <new>
 #include <vector>
 
+#include "engine_host.h"
 #include "radx_hip.h"
+
+using namespace radx_engine;
 
 namespace {
 
@@ -1344,23 +1347,6 @@ __global__ void checksum_kernel(const K* __restrict__ keys, uint64_t n,
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
-thread_local char g_error[256] = "";
-
-int fail(hipError_t e, const char* what) {
-    snprintf(g_error, sizeof(g_error), "%s: %s", what, hipGetErrorString(e));
-    return static_cast<int>(e);
-}
-int bad_arg(const char* what) {
-    snprintf(g_error, sizeof(g_error), "invalid argument: %s", what);
-    return static_cast<int>(hipErrorInvalidValue);
-}
-
-#define RADX_TRY(expr)                                   \
-    do {                                                 \
-        const hipError_t e_ = (expr);                    \
-        if (e_ != hipSuccess) return fail(e_, #expr);    \
-    } while (0)
-
 constexpr uint64_t kMaxElements = 0xffffffffull;  // element indices are 32-bit, as in the reference
 
 // get_blocks_info (shaders-sdk/radix/includes.glsl:162-173) with grid = ceil(n / tile): every
@@ -1411,20 +1397,6 @@ constexpr ScratchLayout layout_for(uint64_t max_n, int key_bytes) {
 struct Timed {
     hipEvent_t start, stop;
     int kind;
-};
-
-class DeviceGuard {
-public:
-    explicit DeviceGuard(int device) {
-        if (hipGetDevice(&prev_) != hipSuccess) prev_ = -1;
-        if (prev_ != device) { status_ = hipSetDevice(device); changed_ = status_ == hipSuccess; }
-    }
-    ~DeviceGuard() { if (changed_ && prev_ >= 0) (void)hipSetDevice(prev_); }
-    hipError_t status() const { return status_; }
-private:
-    int prev_ = -1;
-    bool changed_ = false;
-    hipError_t status_ = hipSuccess;
 };
 
 }  // namespace
@@ -1672,7 +1644,7 @@ int empty_pass(radx_hip_sorter* s, hipStream_t stream) {
 
 extern "C" {
 
-int radx_hip_version(void) { return 400; }
+int radx_hip_version(void) { return 500; }
 
 const char* radx_hip_error_string(void) { return g_error; }
 
@@ -2071,23 +2043,6 @@ int radx_hip_kernel_times(radx_hip_sorter* s, double ms[3], uint64_t launches[3]
 }
 
 namespace {
-// The free functions below take raw device pointers and no sorter handle: each launches on the
-// device that owns its buffer, whatever device is current on the calling thread.
-int device_of(const void* p, int* device) {
-    hipPointerAttribute_t attr;
-    if (hipPointerGetAttributes(&attr, p) != hipSuccess) {
-        (void)hipGetLastError();
-        return bad_arg("buffer is not memory HIP knows (hipMalloc / hipHostMalloc)");
-    }
-    *device = attr.device;
-    return 0;
-}
-#define RADX_ON_DEVICE_OF(ptr)                                     \
-    int dev_ = 0;                                                  \
-    if (const int rc_ = device_of((ptr), &dev_)) return rc_;       \
-    DeviceGuard guard_(dev_);                                      \
-    RADX_TRY(guard_.status())
-
 int log2_or_minus1(uint32_t v) {
     if (v == 0 || (v & (v - 1))) return -1;
     int l = 0;

@@ -1,7 +1,7 @@
 #!/bin/bash
 # Per-kernel registers, LDS and occupancy of the engine's code object (no GPU needed).
 HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
-$HIPCC -O3 -std=c++17 --offload-arch=gfx950 -Iinclude -Rpass-analysis=kernel-resource-usage -c -o /dev/null \
+$HIPCC -O3 -std=c++17 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -Iinclude -Rpass-analysis=kernel-resource-usage -c -o /dev/null \
     ${1:-radx_amd/csrc/radx_hip.hip} 2>&1 | python3 -c '
 import re, sys, subprocess
 cur = {}

@@ -2,8 +2,8 @@
 # Build a named variant of the engine with extra -D flags and print its scatter kernels' resources.
 #   tools/variant.sh <name> [flags...]   ->  radx_amd/lib/libradx_hip_<name>.so
 name=$1; shift
-/opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Iinclude -Wall -Wno-unused-function "$@" -shared \
-    -o radx_amd/lib/libradx_hip_$name.so radx_amd/csrc/radx_hip.hip -Rpass-analysis=kernel-resource-usage 2>&1 | python3 -c '
+/opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Iinclude -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops "$@" -shared \
+    -o radx_amd/lib/libradx_hip_$name.so radx_amd/csrc/radx_hip.hip radx_amd/csrc/radx_beam.hip -Rpass-analysis=kernel-resource-usage 2>&1 | python3 -c '
 import re,sys
 cur=None
 for ln in sys.stdin:
