@@ -5,6 +5,7 @@
 // reordering is radx_hip_permutation's: rows moved by an index.
 #include <hip/hip_runtime.h>
 
+#include <float.h>
 #include <math.h>
 #include <stdint.h>
 #include <string.h>
@@ -51,67 +52,113 @@ __device__ __forceinline__ uint64_t ordered64(double x) {
 __device__ __forceinline__ double from_ordered64(uint64_t o) {
     return __longlong_as_double(static_cast<int64_t>(o ^ ((o >> 63) ? 0x8000000000000000ull : 0xffffffffffffffffull)));
 }
-constexpr uint32_t kLowestFinite = 0x00800000u;  // ordered(-FLT_MAX): everything below is -inf
+constexpr uint32_t kLowestFinite = 0x00800000u;  // ordered(-FLT_MAX): below it is -inf
 
+// The largest of a wave's values, in every lane: within rows of 16 lanes, then across them.
 __device__ __forceinline__ float wave_max(float v) {
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+#define RADX_DPP_MAX(ctrl) \
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), ctrl, 0xf, 0xf, false)))
+    RADX_DPP_MAX(0x111);  // row_shr:1
+    RADX_DPP_MAX(0x112);
+    RADX_DPP_MAX(0x114);
+    RADX_DPP_MAX(0x118);
+    RADX_DPP_MAX(0x142);  // row_bcast:15
+    RADX_DPP_MAX(0x143);  // row_bcast:31
+#undef RADX_DPP_MAX
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+__device__ __forceinline__ uint32_t lanes_before(uint64_t mask) {
+    return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0u));
 }
 __device__ __forceinline__ double wave_sum(double v) {
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
 
-// Elements of one 16-byte vector as floats.
+// Elements of one 16-byte vector as floats; tail(): the first n elements at p, -inf behind them.
 template <typename T> struct Vec;
 template <> struct Vec<float> {
     static constexpr int n = 4;
-    static constexpr int kOrderedBits = 32;  // leading bits of the ordered image that differ between values
-    static __device__ __forceinline__ void unpack(const uint32_t* w, float* f) {
-        for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[i]);
+    static __device__ __forceinline__ void unpack(uint4 r, float* f) {
+        f[0] = __uint_as_float(r.x);
+        f[1] = __uint_as_float(r.y);
+        f[2] = __uint_as_float(r.z);
+        f[3] = __uint_as_float(r.w);
     }
-    static __device__ __forceinline__ float one(const float* p) { return *p; }
+    static __device__ __forceinline__ uint4 tail(const float* p, uint32_t n) {
+        const uint32_t none = 0xff800000u;
+        return uint4{n > 0 ? __float_as_uint(p[0]) : none, n > 1 ? __float_as_uint(p[1]) : none, n > 2 ? __float_as_uint(p[2]) : none, none};
+    }
 };
-template <> struct Vec<BF16> {
+struct Half16 {  // the 16-bit types
     static constexpr int n = 8;
-    static constexpr int kOrderedBits = 16;
-    static __device__ __forceinline__ void unpack(const uint32_t* w, float* f) {
+    static __device__ __forceinline__ uint4 tail16(const uint16_t* p, uint32_t n, uint32_t none) {
+        uint32_t w[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+            w[i] = (2 * i < n ? p[2 * i] : none) | (2 * i + 1 < n ? p[2 * i + 1] : none) << 16;
+        return uint4{w[0], w[1], w[2], w[3]};
+    }
+};
+template <> struct Vec<BF16> : Half16 {
+    static __device__ __forceinline__ void unpack(uint4 r, float* f) {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
         for (int i = 0; i < 4; ++i) {
             f[2 * i] = __uint_as_float(w[i] << 16);
             f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
         }
     }
-    static __device__ __forceinline__ float one(const BF16* p) { return __uint_as_float(static_cast<uint32_t>(p->bits) << 16); }
+    static __device__ __forceinline__ uint4 tail(const BF16* p, uint32_t n) { return tail16(&p->bits, n, 0xff80u); }
 };
-template <> struct Vec<_Float16> {
-    static constexpr int n = 8;
-    static constexpr int kOrderedBits = 19;  // sign, 8 exponent bits of the float, 10 of the fraction
-    static __device__ __forceinline__ void unpack(const uint32_t* w, float* f) {
+template <> struct Vec<_Float16> : Half16 {
+    static __device__ __forceinline__ void unpack(uint4 r, float* f) {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
         for (int i = 0; i < 4; ++i) {
             f[2 * i] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[i])));
             f[2 * i + 1] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[i] >> 16)));
         }
     }
-    static __device__ __forceinline__ float one(const _Float16* p) { return static_cast<float>(*p); }
+    static __device__ __forceinline__ uint4 tail(const _Float16* p, uint32_t n) { return tail16(reinterpret_cast<const uint16_t*>(p), n, 0xfc00u); }
 };
 
-// A threshold that at least k (k <= 256) of 256 ordered values reach, as high as it gets: the k-th
-// largest of them, or a value that exactly k reach.  Every wave computes the same from LDS.
-template <int BITS>
-__device__ __forceinline__ uint32_t reached_by(const uint32_t* v256, uint32_t k) {
+// Counts by distance below the largest, in bins that grow by 2^(1/PER) or so: whatever the scale of the values,
+// the bins up to the k-th one's hold few more than k.
+constexpr uint32_t kBins = 256;
+// The first bin up to which there are k (the last bin if there are fewer), in every lane of a wave.
+__device__ __forceinline__ uint32_t bin_with(const uint32_t* bins, uint32_t k) {
     const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t a0 = v256[lane], a1 = v256[lane + 64], a2 = v256[lane + 128], a3 = v256[lane + 192];
-    uint32_t t = 0;
-    for (int bit = 31; bit >= 32 - BITS; --bit) {
-        const uint32_t c = t | (1u << bit);
-        const uint32_t n = __popcll(__ballot(a0 >= c)) + __popcll(__ballot(a1 >= c)) + __popcll(__ballot(a2 >= c)) +
-                           __popcll(__ballot(a3 >= c));
-        if (n >= k) t = c;
-        if (n == k) break;
-    }
-    // the bits that are alike in all values of one sign
-    if (BITS < 32 && !(t >> 31)) t |= (1u << (32 - BITS)) - 1u;
-    return t;
+    const uint4 c = reinterpret_cast<const uint4*>(bins)[lane];
+    const uint32_t c1 = c.x + c.y, c2 = c1 + c.z, c3 = c2 + c.w;
+    uint32_t upto = c3;
+#define RADX_DPP_ADD(ctrl, rows) \
+    upto += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(upto), ctrl, rows, 0xf, false))
+    RADX_DPP_ADD(0x111, 0xf);  // row_shr:1
+    RADX_DPP_ADD(0x112, 0xf);
+    RADX_DPP_ADD(0x114, 0xf);
+    RADX_DPP_ADD(0x118, 0xf);
+    RADX_DPP_ADD(0x142, 0xa);  // row_bcast:15 into rows 1 and 3
+    RADX_DPP_ADD(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
+#undef RADX_DPP_ADD
+    const uint64_t enough = __ballot(upto >= k);
+    if (!enough) return kBins - 1;
+    const uint32_t before = upto - c3;
+    const uint32_t at = 4 * lane + (before + c.x >= k ? 0 : before + c1 >= k ? 1 : before + c2 >= k ? 2 : 3);
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(at), __ffsll(static_cast<unsigned long long>(enough)) - 1));
+}
+// Bins of whole-number distances: 0, and eight for every power of two.
+__device__ __forceinline__ uint32_t bin_of(uint32_t distance) {
+    if (distance < 8) return distance;
+    const uint32_t top = 31 - __clz(distance);
+    return (top - 2) * 8 + ((distance >> (top - 3)) & 7u);
+}
+// The largest distance that a bin holds.
+__device__ __forceinline__ uint32_t end_of_bin(uint32_t bin) {
+    if (bin < 8) return bin;
+    const uint32_t top = bin / 8 + 2;
+    const uint64_t end = (8ull + (bin & 7u) + 1) << (top - 3);
+    return end > 0xffffffffull ? 0xffffffffu : static_cast<uint32_t>(end) - 1u;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -120,12 +167,12 @@ __device__ __forceinline__ uint32_t reached_by(const uint32_t* v256, uint32_t k)
 // score(row, token) = cum[row] + ((x - M) - log sum exp(x - M)): within a row the order of the scores
 // is the order of the logits, so a slice can be searched for its own k best before M and the sum
 // are known.  A slice leaves its maximum, its sum of exponentials relative to that maximum, and its
-// k best logits, sorted.
+// k best logits.
 struct SliceInfo {
     double sum;      // of exp(x - max)
     uint64_t head;   // the slice's best entry (0: none)
     float max;
-    uint32_t count;  // entries left in best[]
+    uint32_t pad;
 };
 
 struct SelectArgs {
@@ -140,7 +187,7 @@ struct SelectArgs {
     uint32_t beams, vocab, k;
     uint32_t slices, tiles_per_slice;
     SliceInfo* info;            // [row][slice]
-    uint64_t* best;             // [row][slice][k]: ordered logit, then ~token
+    uint64_t* best;             // [row][slice][k]: ordered logit, then ~token; 0: none
     float* scores;
     int32_t* parents;
     int32_t* tokens;
@@ -149,34 +196,115 @@ struct SelectArgs {
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
+// Orders a wave's LDS traffic between its lanes: the wave runs in step and its LDS operations are
+// done in order, so only the compiler has to be held back.
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+constexpr uint32_t kWaveList = 512;  // entries a wave can hold while it looks through a tile
+
+// The k-th largest of list[0..n), n >= k; the keys are unique and none is 0.  For lists that grew too long only.
+__device__ __forceinline__ uint64_t kth_key(const uint64_t* list, uint32_t n, uint32_t k) {
+    const uint32_t lane = threadIdx.x & 63u;
+    uint64_t high = 0, low = ~0ull;
+    for (uint32_t at = lane; at < n; at += 64) {
+        high = max(high, list[at]);
+        low = min(low, list[at]);
+    }
+    for (int o = 32; o; o >>= 1) {
+        high = max(high, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(high), o)));
+        low = min(low, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(low), o)));
+    }
+    if (high == low) return high;
+    // bits in which all agree need no step
+    const int alike = __clzll(static_cast<long long>(high ^ low));
+    uint64_t t = alike ? high & ~(~0ull >> alike) : 0;
+#pragma unroll 1
+    for (int bit = 63 - alike; bit >= 0; --bit) {
+        const uint64_t c = t | (1ull << bit);
+        uint32_t m = 0;
+#pragma unroll
+        for (uint32_t r = 0; r < kWaveList / 64; ++r) {
+            if (r * 64 >= n) break;
+            m += __popcll(__ballot(r * 64 + lane < n && list[r * 64 + lane] >= c));
+        }
+        if (m >= k) t = c;
+        if (m == k) break;
+    }
+    return t;
+}
+
+// Leaves the entries of list[0..n) that reach t, in front.
+__device__ __forceinline__ uint32_t keep_from(uint64_t* list, uint32_t n, uint64_t t) {
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t kept = 0;
+    for (uint32_t at = 0; at < n; at += 64) {
+        const uint64_t key = at + lane < n ? list[at + lane] : 0;
+        const uint64_t mask = __ballot(key != 0 && key >= t);
+        wave_fence();
+        if (key != 0 && key >= t) list[kept + lanes_before(mask)] = key;
+        wave_fence();
+        kept += __popcll(mask);
+    }
+    return kept;
+}
+
 constexpr int kVecs = 4;  // 16-byte vectors a thread holds: a tile is 16 KiB of logits
 template <typename T> constexpr uint32_t tile_of() { return kThreads * kVecs * Vec<T>::n; }
 
-// Entries a workgroup can stage between two prunings.  A tile holds at most 32 elements a thread; of those above the
-// threshold at most k - 1 threads have any, and of those equal to it at most k are taken.
-constexpr uint32_t stage_entries(uint32_t k) { return 33 * k < 1024 ? 1024 : 33 * k; }
+// A thread's part of a tile, as it came from memory.  What lies behind the row is -inf.
+template <typename T, bool MASKED>
+struct TilePart {
+    uint4 raw[kVecs];
+    uint8_t bits[kVecs];
 
-// The k largest of from[0..n_from) and stage[0..n) into to[], sorted.  Keys are unique: an entry's place is
-// the number of larger ones.
-__device__ __forceinline__ uint32_t prune(const uint64_t* from, uint32_t n_from, const uint64_t* stage, uint32_t n, uint64_t* to, uint32_t k) {
-    const uint32_t all = n_from + n;
-    for (uint32_t i = threadIdx.x; i < all; i += kThreads) {
-        const uint64_t key = i < n_from ? from[i] : stage[i - n_from];
-        uint32_t above = 0;
-        for (uint32_t j = 0; j < n_from; ++j) above += from[j] > key;
-        for (uint32_t j = 0; j < n; ++j) above += stage[j] > key;
-        if (above < k) to[above] = key;
+    __device__ __forceinline__ void load(const T* x, const uint8_t* mask, uint32_t at, uint32_t vocab) {
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j, at += 64 * Vec<T>::n) {
+            if (at + Vec<T>::n <= vocab) {
+                const Bytes16 b = *reinterpret_cast<const Bytes16*>(x + at);
+                raw[j] = uint4{b.w[0], b.w[1], b.w[2], b.w[3]};
+            } else {
+                raw[j] = Vec<T>::tail(x + at, at < vocab ? vocab - at : 0);
+            }
+            if (MASKED) bits[j] = at < vocab ? mask[at >> 3] : 0;
+        }
     }
-    __syncthreads();
-    return all < k ? all : k;
+    __device__ __forceinline__ void unpack(uint32_t at, float* f) const {
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j, at += 64 * Vec<T>::n) {
+            Vec<T>::unpack(raw[j], f + j * Vec<T>::n);
+            if (MASKED) {
+                const uint32_t b = static_cast<uint32_t>(bits[j]) >> (at & 7u);
+#pragma unroll
+                for (int e = 0; e < Vec<T>::n; ++e) f[j * Vec<T>::n + e] = (b >> e) & 1u ? f[j * Vec<T>::n + e] : -INFINITY;
+            }
+        }
+    }
+};
+
+// The number of entries in a workgroup's lists that are larger than key.
+__device__ __forceinline__ uint32_t larger(const uint64_t (*lists)[kWaveList], const uint32_t* listed, uint64_t key) {
+    uint32_t above = 0;
+    for (int w = 0; w < kWaves; ++w) {
+        const uint32_t n = listed[w];
+#pragma unroll 4
+        for (uint32_t j = 0; j < n; ++j) above += lists[w][j] > key;
+    }
+    return above;
 }
 
+// Candidates are the elements that reach a threshold which k elements are known to reach: in the first tile
+// one that k of its 1024 vectors' maxima reach (few more do, by their counts), then the k-th best of that
+// tile.  Every wave collects its own in a list, so nothing waits inside the loop over the other tiles.
 template <typename T, bool MASKED>
-__global__ __launch_bounds__(kThreads) void beam_slice_kernel(SelectArgs a) {
-    extern __shared__ uint64_t stage[];
-    __shared__ uint64_t kept_in_turn[2][kMaxK];
-    __shared__ uint32_t lane_max[kThreads];
-    __shared__ uint32_t staged, equals[kWaves];
+__global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
+    __shared__ uint64_t lists[kWaves][kWaveList];
+    __shared__ uint64_t block_kth;
+    __shared__ __attribute__((aligned(16))) uint32_t bins[kBins];
+    __shared__ uint32_t listed[kWaves], wave_top[kWaves];
     __shared__ float wave_ref[kWaves];
     __shared__ double wave_total[kWaves];
     constexpr int V = Vec<T>::n;
@@ -184,8 +312,10 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(SelectArgs a) {
 
     const uint32_t row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t k = a.k;
     SliceInfo* info = a.info + static_cast<size_t>(row) * a.slices + slice;
     if (!finite(a.cum[row]) || (a.finished && a.finished[row])) {
+        // nothing is looked up in a row that offers nothing by its logits
         if (threadIdx.x == 0) *info = SliceInfo{0.0, 0, -INFINITY, 0};
         return;
     }
@@ -193,39 +323,47 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(SelectArgs a) {
     const uint8_t* mask = MASKED ? reinterpret_cast<const uint8_t*>(a.allowed + static_cast<int64_t>(row) * a.allowed_stride) : nullptr;
     const uint32_t first = slice * a.tiles_per_slice * kTile;
     const uint32_t last = min(a.vocab, first + a.tiles_per_slice * kTile);
+    const uint32_t mine = wave * (kTile / kWaves) + lane * V;
 
+    uint64_t* list = lists[wave];
+    uint32_t n = 0;              // entries in it
+    uint64_t kth = 0;            // an entry has to reach it
+    float thr = -FLT_MAX;        // and so an element this
     double sum = 0.0;            // this lane's share, relative to ref
     float ref = -INFINITY;       // the wave's maximum so far
-    uint64_t* kept = kept_in_turn[0];
-    uint64_t* spare = kept_in_turn[1];
-    uint32_t n_kept = 0;
-    float floor_x = -INFINITY;   // an element has to be above it: the k-th best so far
-    if (threadIdx.x == 0) staged = 0;
 
+    TilePart<T, MASKED> next;
+    next.load(x, mask, first + mine, a.vocab);
     for (uint32_t tile = first; tile < last; tile += kTile) {
         float f[kVecs * V];
+        next.unpack(tile + mine, f);
+        if (tile + kTile < last) next.load(x, mask, tile + kTile + mine, a.vocab);
+        float top[kVecs];
+        float most = -INFINITY;
 #pragma unroll
         for (int j = 0; j < kVecs; ++j) {
-            const uint32_t at = tile + (j * kThreads + threadIdx.x) * V;
-            uint32_t bits = ~0u;
-            if (at + V <= a.vocab) {
-                const Bytes16 b = *reinterpret_cast<const Bytes16*>(x + at);
-                Vec<T>::unpack(b.w, f + j * V);
-                if (MASKED) bits = mask[at >> 3] >> (at & 7u);
-            } else {
-                for (int e = 0; e < V; ++e) f[j * V + e] = at + e < a.vocab ? Vec<T>::one(x + at + e) : -INFINITY;
-                if (MASKED && at < a.vocab) bits = mask[at >> 3] >> (at & 7u);
-            }
-            if (MASKED)
-                for (int e = 0; e < V; ++e) f[j * V + e] = (bits >> e) & 1u ? f[j * V + e] : -INFINITY;
-        }
-        float top = f[0];
+            top[j] = f[j * V];
 #pragma unroll
-        for (int e = 1; e < kVecs * V; ++e) top = fmaxf(top, f[e]);
+            for (int e = 1; e < V; ++e) top[j] = fmaxf(top[j], f[j * V + e]);
+            most = fmaxf(most, top[j]);
+        }
+        if (tile == first) {
+            const float high = wave_max(most);
+            if (lane == 0) wave_top[wave] = ordered(high);
+            bins[threadIdx.x] = 0;
+            __syncthreads();
+            const uint32_t o = max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3]));
+#pragma unroll
+            for (int j = 0; j < kVecs; ++j)
+                if (top[j] >= thr) atomicAdd(&bins[bin_of(o - ordered(top[j]))], 1u);
+            __syncthreads();
+            const uint32_t reach = end_of_bin(bin_with(bins, k));
+            if (o > kLowestFinite && o - kLowestFinite > reach) thr = from_ordered(o - reach);
+        }
 
         // sum of exponentials relative to the wave's maximum; 2^(d * log2 e) with log2 e in two parts
-        const float new_ref = fmaxf(ref, wave_max(top));
-        if (new_ref != ref) {
+        if (__any(most > ref)) {
+            const float new_ref = fmaxf(ref, wave_max(most));
             if (ref > -INFINITY) sum *= exp(static_cast<double>(ref) - static_cast<double>(new_ref));
             ref = new_ref;
         }
@@ -242,119 +380,93 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(SelectArgs a) {
             sum += static_cast<double>(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])));
         }
 
-        // candidates: everything above the k-th best so far; a threshold from the threads' maxima where that is too much
-        __syncthreads();  // staged is 0
-        float above = floor_x;
-        bool or_equal = false;
-        if (n_kept < a.k) {
-            lane_max[threadIdx.x] = ordered(top);
-            __syncthreads();
-            const uint32_t t = reached_by<Vec<T>::kOrderedBits>(lane_max, a.k);
-            above = t < kLowestFinite ? -INFINITY : from_ordered(t);
-            or_equal = t >= kLowestFinite;
-        }
-        const uint32_t room = stage_entries(a.k);
-        if (top > above || (or_equal && top == above))
+        while (__any(most >= thr)) {
+            uint32_t m = n;
+            bool over = false;
 #pragma unroll
-            for (int j = 0; j < kVecs; ++j)
+            for (int j = 0; j < kVecs; ++j) {
+                if (!__any(top[j] >= thr)) continue;
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    const float v = f[j * V + e];
-                    if (v > above || (or_equal && v == above)) {
-                        const uint32_t at = atomicAdd(&staged, 1u);
-                        const uint32_t token = tile + (j * kThreads + threadIdx.x) * V + e;
-                        if (at < room) stage[at] = static_cast<uint64_t>(ordered(v)) << 32 | (0xffffffffu - token);
+                    float v = f[j * V + e];
+                    if (!__any(v >= thr)) continue;
+                    uint32_t token = tile + mine;
+                    asm volatile("" : "+v"(v), "+v"(token));  // the keys of all elements would be made ahead, in a register each
+                    const uint64_t key = static_cast<uint64_t>(ordered(v)) << 32 | ~(token + j * 64 * V + e);
+                    const bool in = v >= thr && key >= kth;
+                    const uint64_t who = __ballot(in);
+                    const uint32_t c = __popcll(who);
+                    over |= m + c > kWaveList;
+                    if (m + c <= kWaveList) {
+                        if (in) list[m + lanes_before(who)] = key;
+                        m += c;
                     }
                 }
-        __syncthreads();
-        uint32_t n = staged;
-        if (n > room) {
-            // too many are equal to the threshold (or pass it): take those above a threshold first,
-            // then the first k of those equal to it, in order of their tokens
-            __syncthreads();
-            if (threadIdx.x == 0) staged = 0;
-            float cut = above;
-            if (!or_equal) {
-                float fresh = -INFINITY;
-                for (int e = 0; e < kVecs * V; ++e) fresh = fmaxf(fresh, f[e]);
-                lane_max[threadIdx.x] = ordered(fresh);
-                __syncthreads();
-                const uint32_t t = reached_by<Vec<T>::kOrderedBits>(lane_max, a.k);
-                cut = t < kLowestFinite ? -INFINITY : fmaxf(above, from_ordered(t));
             }
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < kVecs; ++j)
-#pragma unroll
-                for (int e = 0; e < V; ++e)
-                    if (f[j * V + e] > cut) {
-                        const uint32_t at = atomicAdd(&staged, 1u);
-                        const uint32_t token = tile + (j * kThreads + threadIdx.x) * V + e;
-                        if (at < room) stage[at] = static_cast<uint64_t>(ordered(f[j * V + e])) << 32 | (0xffffffffu - token);
-                    }
-            uint32_t taken = 0;
-            if (cut > above || or_equal)
-#pragma unroll
-                for (int j = 0; j < kVecs; ++j) {
-                    uint32_t mine = 0;
-#pragma unroll
-                    for (int e = 0; e < V; ++e) mine += f[j * V + e] == cut;
-                    uint32_t before = mine;
-                    for (int o = 1; o < 64; o <<= 1) {
-                        const uint32_t u = __shfl_up(before, o);
-                        if (lane >= static_cast<uint32_t>(o)) before += u;
-                    }
-                    if (lane == 63u) equals[wave] = before;
-                    before -= mine;
-                    __syncthreads();
-                    uint32_t all = 0;
-                    for (uint32_t w = 0; w < kWaves; ++w) {
-                        if (w < wave) before += equals[w];
-                        all += equals[w];
-                    }
-                    before += taken;
-#pragma unroll
-                    for (int e = 0; e < V; ++e)
-                        if (f[j * V + e] == cut) {
-                            if (before < a.k) {
-                                const uint32_t at = atomicAdd(&staged, 1u);
-                                const uint32_t token = tile + (j * kThreads + threadIdx.x) * V + e;
-                                if (at < room) stage[at] = static_cast<uint64_t>(ordered(cut)) << 32 | (0xffffffffu - token);
-                            }
-                            ++before;
-                        }
-                    taken += all;
-                    __syncthreads();
-                }
-            __syncthreads();
-            n = min(staged, room);
+            wave_fence();
+            if (!over) {
+                n = m;
+                break;
+            }
+            // more than the list holds: with the k-th best of what it holds as the threshold, this tile's
+            // entries are taken again (n <= 192 and k <= 128 of over 448, so every turn leaves many out)
+            kth = kth_key(list, m, k);
+            thr = from_ordered(static_cast<uint32_t>(kth >> 32));
+            wave_fence();
         }
-        if (n) {
-            n_kept = prune(kept, n_kept, stage, n, spare, a.k);
-            uint64_t* const was = kept;
-            kept = spare;
-            spare = was;
-            if (n_kept == a.k) floor_x = from_ordered(static_cast<uint32_t>(kept[a.k - 1] >> 32));
-            if (threadIdx.x == 0) staged = 0;
+        if (n > k + 64) {
+            kth = max(kth, kth_key(list, n, k));
+            thr = from_ordered(static_cast<uint32_t>(kth >> 32));
+            n = keep_from(list, n, kth);
+        }
+        if (tile == first && tile + kTile < last) {
+            if (threadIdx.x == 0) block_kth = 0;
+            if (lane == 0) listed[wave] = n;
+            __syncthreads();
+            for (uint32_t i = lane; i < n; i += 64)
+                if (larger(lists, listed, list[i]) == k - 1) block_kth = list[i];
+            __syncthreads();
+            if (block_kth > kth) {
+                kth = block_kth;
+                thr = from_ordered(static_cast<uint32_t>(kth >> 32));
+            }
         }
     }
 
     const double total = wave_sum(sum);
     if (lane == 0) {
+        listed[wave] = n;
         wave_ref[wave] = ref;
         wave_total[wave] = total;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        float m = wave_ref[0];
-        for (int w = 1; w < kWaves; ++w) m = fmaxf(m, wave_ref[w]);
-        double s = 0.0;
-        for (int w = 0; w < kWaves; ++w)
-            s += wave_ref[w] > -INFINITY ? wave_total[w] * exp(static_cast<double>(wave_ref[w]) - static_cast<double>(m)) : wave_total[w];
-        *info = SliceInfo{s, n_kept ? kept[0] : 0, m, n_kept};
+    // the four lists as one, sorted: an entry's place is the number of larger ones
+    uint64_t* best = a.best + (static_cast<size_t>(row) * a.slices + slice) * k;
+    uint32_t all = 0;
+    for (int w = 0; w < kWaves; ++w) all += listed[w];
+    for (uint32_t i = lane; i < n; i += 64) {
+        const uint64_t key = list[i];
+        const uint32_t above = larger(lists, listed, key);
+        if (above < k) best[above] = key;
+        if (above == 0) info->head = key;
     }
-    uint64_t* best = a.best + (static_cast<size_t>(row) * a.slices + slice) * a.k;
-    for (uint32_t i = threadIdx.x; i < n_kept; i += kThreads) best[i] = kept[i];
+    for (uint32_t i = all + threadIdx.x; i < k; i += kThreads) best[i] = 0;
+    if (all == 0 && threadIdx.x == 0) info->head = 0;
+    if (wave == 0) {
+        float m = fmaxf(fmaxf(wave_ref[0], wave_ref[1]), fmaxf(wave_ref[2], wave_ref[3]));
+        double s = 0.0;
+        if (lane < kWaves) {
+            // a wave without a number above -inf has no maximum to scale by; its sum is 0, or a NaN to be passed on
+            s = wave_total[lane];
+            if (wave_ref[lane] > -INFINITY) s *= exp(static_cast<double>(wave_ref[lane]) - static_cast<double>(m));
+        }
+        s += __shfl_xor(s, 1);
+        s += __shfl_xor(s, 2);
+        if (lane == 0) {
+            info->sum = s;
+            info->max = m;
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -363,6 +475,7 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(SelectArgs a) {
 // The rows' maxima and sums are joined from their slices, every slice's entries get their scores in
 // 64 bits, and the k best come out in the order (score down, beam up, logit down, token up).
 // Within a beam that is the slices' own order.
+constexpr uint32_t kMergeThreads = 1024;
 constexpr uint32_t kMergeStage = 1024;
 
 struct Entry {
@@ -375,18 +488,20 @@ __device__ __forceinline__ bool better(const Entry& p, const Entry& q) {
 
 struct RowBase {
     double top, log_sum, cum;
-    int live;
 };
 
-__device__ __forceinline__ Entry entry_of(const RowBase& r, uint32_t beam, uint64_t key) {
-    const uint32_t o = static_cast<uint32_t>(key >> 32), token = 0xffffffffu - static_cast<uint32_t>(key);
-    const double s = r.cum + ((static_cast<double>(from_ordered(o)) - r.top) - r.log_sum);
-    return Entry{ordered64(s), static_cast<uint64_t>(beam) << 56 | static_cast<uint64_t>(~o) << 24 | token};
+__device__ __forceinline__ double score_of(const RowBase& r, uint64_t key) {
+    return r.cum + ((static_cast<double>(from_ordered(static_cast<uint32_t>(key >> 32))) - r.top) - r.log_sum);
 }
 
+__device__ __forceinline__ Entry entry_of(const RowBase& r, uint32_t beam, uint64_t key) {
+    const uint32_t o = static_cast<uint32_t>(key >> 32), token = ~static_cast<uint32_t>(key);
+    return Entry{ordered64(score_of(r, key)), static_cast<uint64_t>(beam) << 56 | static_cast<uint64_t>(~o) << 24 | token};
+}
+// The k best of from[0..n_from) and stage[0..n) into to[], sorted: an entry's place is the number of better ones.
 __device__ __forceinline__ uint32_t prune(const Entry* from, uint32_t n_from, const Entry* stage, uint32_t n, Entry* to, uint32_t k) {
     const uint32_t all = n_from + n;
-    for (uint32_t i = threadIdx.x; i < all; i += kThreads) {
+    for (uint32_t i = threadIdx.x; i < all; i += kMergeThreads) {
         const Entry e = i < n_from ? from[i] : stage[i - n_from];
         uint32_t above = 0;
         for (uint32_t j = 0; j < n_from; ++j) above += better(from[j], e);
@@ -397,67 +512,112 @@ __device__ __forceinline__ uint32_t prune(const Entry* from, uint32_t n_from, co
     return all < k ? all : k;
 }
 
-__global__ __launch_bounds__(kThreads) void beam_merge_kernel(SelectArgs a) {
+// Bins of scores by their distance below the best one, four for every power of two from 2^-44 up.
+__device__ __forceinline__ uint32_t bin_of(double best, double score) {
+    const uint32_t b = __float_as_uint(static_cast<float>(best - score)) >> 21;  // exponent and two bits of the fraction
+    constexpr uint32_t kLow = (127 - 44) * 4;
+    return b <= kLow ? 0 : min(b - kLow, kBins - 1);
+}
+
+__global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(SelectArgs a) {
+    extern __shared__ uint32_t heads[];  // bin of every list's best entry, then the lists that are looked into
     __shared__ RowBase base[kMaxBeams];
     __shared__ Entry kept_in_turn[2][kMaxK];
     __shared__ Entry stage[kMergeStage];
-    __shared__ uint32_t lane_max[kThreads];
-    __shared__ uint32_t staged;
+    __shared__ __attribute__((aligned(16))) uint32_t bins[kBins];
+    __shared__ double wave_best[kMergeThreads / 64];
+    __shared__ uint32_t staged, looked;
     const uint32_t item = blockIdx.x;
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t lane = threadIdx.x & 63u;
     const uint32_t lists = a.beams * a.slices;
     const SliceInfo* info = a.info + static_cast<size_t>(item) * lists;
     const uint64_t* best = a.best + static_cast<size_t>(item) * lists * a.k;
+    uint32_t* look = heads + lists;
 
-    if (threadIdx.x == 0) staged = 0;
-    for (uint32_t i = wave; i < a.beams; i += kWaves) {
-        const uint32_t row = item * a.beams + i;
+    if (threadIdx.x == 0) staged = looked = 0;
+    if (threadIdx.x < kBins) bins[threadIdx.x] = 0;
+    __syncthreads();
+    // rows: a group of lanes each, a power of two that covers the slices
+    uint32_t group = 1;
+    while (group < a.slices && group < 64) group <<= 1;
+    const uint32_t first = threadIdx.x & (group - 1u);
+    double top = -INFINITY;  // the best score among this thread's lists
+    for (uint32_t beam = threadIdx.x / group; beam < a.beams; beam += kMergeThreads / group) {
+        const uint32_t row = item * a.beams + beam;
         const float cum = a.cum[row];
         const bool ended = a.finished && a.finished[row];
+        const SliceInfo* mine = info + beam * a.slices;
         float m = -INFINITY;
-        for (uint32_t s = lane; s < a.slices; s += 64) m = fmaxf(m, info[i * a.slices + s].max);
-        m = wave_max(m);
+        for (uint32_t s = first; s < a.slices; s += group) m = fmaxf(m, mine[s].max);
+        for (uint32_t o = group >> 1; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
         double sum = 0.0;
-        for (uint32_t s = lane; s < a.slices; s += 64) {
-            const SliceInfo p = info[i * a.slices + s];
-            if (p.max > -INFINITY || !(p.sum == 0.0)) sum += p.sum * exp(static_cast<double>(p.max) - static_cast<double>(m));
+        for (uint32_t s = first; s < a.slices; s += group) {
+            const float ms = mine[s].max;
+            const double p = mine[s].sum;
+            if (ms > -INFINITY || !(p == 0.0)) sum += p * exp(static_cast<double>(ms) - static_cast<double>(m));
         }
-        sum = wave_sum(sum);
-        if (lane == 0) {
-            // a NaN or +inf among the allowed logits has made the sum a NaN
-            const bool live = !ended && finite(cum) && finite(m) && sum > 0.0 && sum < INFINITY;
-            base[i] = RowBase{a.normalize ? static_cast<double>(m) : 0.0, a.normalize ? log(sum) : 0.0, static_cast<double>(cum), live};
-        }
-        if (ended && finite(cum) && lane == 0) {
-            const uint32_t at = atomicAdd(&staged, 1u);
-            stage[at] = Entry{ordered64(cum), static_cast<uint64_t>(i) << 56 | static_cast<uint32_t>(a.end_token)};
+        for (uint32_t o = group >> 1; o; o >>= 1) sum += __shfl_xor(sum, o);
+        // a NaN or +inf among the allowed logits has made the sum a NaN
+        const bool live = !ended && finite(cum) && finite(m) && sum > 0.0 && sum < INFINITY;
+        const RowBase r{a.normalize ? static_cast<double>(m) : 0.0, a.normalize ? log(sum) : 0.0, live ? static_cast<double>(cum) : -INFINITY};
+        if (live) top = fmax(top, score_of(r, static_cast<uint64_t>(ordered(m)) << 32));
+        if (first == 0) {
+            base[beam] = r;
+            if (ended && finite(cum)) {
+                stage[atomicAdd(&staged, 1u)] = Entry{ordered64(cum), static_cast<uint64_t>(beam) << 56 | static_cast<uint32_t>(a.end_token)};
+                top = fmax(top, static_cast<double>(cum));
+            }
         }
     }
+    for (int o = 32; o; o >>= 1) top = fmax(top, __shfl_xor(top, o));
+    if (lane == 0) wave_best[threadIdx.x >> 6] = top;
     __syncthreads();
+    for (uint32_t w = 0; w < kMergeThreads / 64; ++w) top = fmax(top, wave_best[w]);
 
-    // a threshold that k heads of lists (or finished beams) reach
-    uint32_t top = threadIdx.x < staged ? static_cast<uint32_t>(stage[threadIdx.x].score >> 32) : 0;
-    for (uint32_t l = threadIdx.x; l < lists; l += kThreads) {
-        const uint32_t beam = l / a.slices;
-        if (base[beam].live && info[l].count) top = max(top, static_cast<uint32_t>(entry_of(base[beam], beam, info[l].head).score >> 32));
-    }
-    lane_max[threadIdx.x] = top;
-    __syncthreads();
-    const uint32_t cut = reached_by<32>(lane_max, a.k);
+    // which lists: those whose best entry is among the k best of all lists' best ones
     const uint32_t ended_beams = staged;
-    __syncthreads();
-
-    for (uint32_t l = wave; l < lists; l += kWaves) {
-        const uint32_t beam = l / a.slices;
-        if (!base[beam].live) continue;
-        const uint32_t count = info[l].count;
-        if (!count || static_cast<uint32_t>(entry_of(base[beam], beam, info[l].head).score >> 32) < cut) continue;
-        for (uint32_t j = lane; j < count; j += 64) {
-            const Entry e = entry_of(base[beam], beam, best[static_cast<size_t>(l) * a.k + j]);
-            if (static_cast<uint32_t>(e.score >> 32) < cut) continue;
-            const uint32_t at = atomicAdd(&staged, 1u);
-            if (at < kMergeStage) stage[at] = e;
+    const bool all_lists = lists * a.k <= 2 * kMergeThreads;
+    uint32_t n_look = lists;
+    if (!all_lists) {
+        for (uint32_t l = threadIdx.x; l < lists; l += kMergeThreads) {
+            const uint32_t beam = l / a.slices;
+            const bool live = base[beam].cum > -INFINITY;
+            const uint64_t head = live ? info[l].head : 0;
+            const uint32_t bin = head ? bin_of(top, score_of(base[beam], head)) : kBins;
+            heads[l] = bin;
+            if (bin < kBins) atomicAdd(&bins[bin], 1u);
         }
+        if (threadIdx.x < ended_beams) atomicAdd(&bins[bin_of(top, from_ordered64(stage[threadIdx.x].score))], 1u);
+        __syncthreads();
+        const uint32_t upto = bin_with(bins, a.k);
+        __syncthreads();
+        for (uint32_t l = threadIdx.x; l < lists; l += kMergeThreads)
+            if (heads[l] <= upto) look[atomicAdd(&looked, 1u)] = l;
+        if (threadIdx.x < kBins) bins[threadIdx.x] = 0;
+        __syncthreads();
+        n_look = looked;
+    }
+    // which entries: those among the k best by the same count
+    const uint32_t some = n_look * a.k;
+    auto entry_at = [&](uint32_t i, uint32_t& beam) -> uint64_t {
+        const uint32_t which = i / a.k, l = all_lists ? which : look[which];
+        beam = l / a.slices;
+        return base[beam].cum > -INFINITY ? best[static_cast<size_t>(l) * a.k + (i - which * a.k)] : 0;
+    };
+    for (uint32_t i = threadIdx.x; i < some; i += kMergeThreads) {
+        uint32_t beam;
+        const uint64_t key = entry_at(i, beam);
+        if (key) atomicAdd(&bins[bin_of(top, score_of(base[beam], key))], 1u);
+    }
+    if (threadIdx.x < ended_beams) atomicAdd(&bins[bin_of(top, from_ordered64(stage[threadIdx.x].score))], 1u);
+    __syncthreads();
+    const uint32_t upto = bin_with(bins, a.k);
+    for (uint32_t i = threadIdx.x; i < some; i += kMergeThreads) {
+        uint32_t beam;
+        const uint64_t key = entry_at(i, beam);
+        if (!key || bin_of(top, score_of(base[beam], key)) > upto) continue;
+        const uint32_t at = atomicAdd(&staged, 1u);
+        if (at < kMergeStage) stage[at] = entry_of(base[beam], beam, key);
     }
     __syncthreads();
     const Entry* kept = kept_in_turn[0];
@@ -469,14 +629,15 @@ __global__ __launch_bounds__(kThreads) void beam_merge_kernel(SelectArgs a) {
         n_kept = prune(kept, 0, stage, ended_beams, kept_in_turn[0], a.k);
         uint32_t turn = 1;
         const uint32_t step = kMergeStage / a.k;
-        for (uint32_t l0 = 0; l0 < lists; l0 += step) {
+        for (uint32_t l0 = 0; l0 < n_look; l0 += step) {
             if (threadIdx.x == 0) staged = 0;
             __syncthreads();
-            const uint32_t some = min(step, lists - l0);
-            for (uint32_t i = threadIdx.x; i < some * a.k; i += kThreads) {
-                const uint32_t l = l0 + i / a.k, j = i % a.k, beam = l / a.slices;
-                if (!base[beam].live || j >= info[l].count) continue;
-                const Entry e = entry_of(base[beam], beam, best[static_cast<size_t>(l) * a.k + j]);
+            const uint32_t now = min(step, n_look - l0) * a.k;
+            for (uint32_t i = threadIdx.x; i < now; i += kMergeThreads) {
+                uint32_t beam;
+                const uint64_t key = entry_at(l0 * a.k + i, beam);
+                if (!key || bin_of(top, score_of(base[beam], key)) > upto) continue;
+                const Entry e = entry_of(base[beam], beam, key);
                 if (n_kept == a.k && !better(e, kept[a.k - 1])) continue;
                 stage[atomicAdd(&staged, 1u)] = e;
             }
@@ -487,7 +648,7 @@ __global__ __launch_bounds__(kThreads) void beam_merge_kernel(SelectArgs a) {
         }
     }
 
-    for (uint32_t i = threadIdx.x; i < a.k; i += kThreads) {
+    for (uint32_t i = threadIdx.x; i < a.k; i += kMergeThreads) {
         const size_t at = static_cast<size_t>(item) * a.k + i;
         float score = -INFINITY;
         int32_t parent = -1, token = -1;
@@ -641,7 +802,7 @@ namespace {
 
 // Slices of all rows of a call that long vocabularies are cut into: enough workgroups to fill 256
 // CUs several times over, and few enough that their k best stay a small part of what is read.
-constexpr uint64_t kSlicesWanted = 4096;
+constexpr uint64_t kSlicesWanted = 1024;
 
 struct Cut {
     uint32_t tiles_per_slice, slices;
@@ -675,10 +836,9 @@ bool overlap(const void* p, uint64_t p_bytes, const void* q, uint64_t q_bytes) {
 
 template <typename T>
 void launch_slices(const SelectArgs& a, uint32_t rows, hipStream_t stream) {
-    const size_t lds = stage_entries(a.k) * sizeof(uint64_t);
     const dim3 grid(rows * a.slices);
-    if (a.allowed) hipLaunchKernelGGL((beam_slice_kernel<T, true>), grid, dim3(kThreads), lds, stream, a);
-    else hipLaunchKernelGGL((beam_slice_kernel<T, false>), grid, dim3(kThreads), lds, stream, a);
+    if (a.allowed) hipLaunchKernelGGL((beam_slice_kernel<T, true>), grid, dim3(kThreads), 0, stream, a);
+    else hipLaunchKernelGGL((beam_slice_kernel<T, false>), grid, dim3(kThreads), 0, stream, a);
 }
 
 }  // namespace
@@ -783,7 +943,7 @@ int radx_hip_beam_select(radx_hip_beam* h, const radx_hip_beam_select_args* s, v
     else if (s->dtype == RADX_HIP_BF16) launch_slices<BF16>(a, n_rows, st);
     else launch_slices<_Float16>(a, n_rows, st);
     RADX_TRY(hipGetLastError());
-    hipLaunchKernelGGL(beam_merge_kernel, dim3(s->batch), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL(beam_merge_kernel, dim3(s->batch), dim3(kMergeThreads), 2 * sizeof(uint32_t) * a.beams * a.slices, st, a);
     RADX_TRY(hipGetLastError());
     return 0;
 }
