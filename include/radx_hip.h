@@ -329,7 +329,7 @@ int radx_hip_beam_select(radx_hip_beam* h, const radx_hip_beam_select_args* args
  *
  *   dst row b * dst_beams + j = src row b * src_beams + parents[b][j]
  *
- * parents[batch][k] on the device, k <= 64; where a parent is < 0 or >= src_beams the row is left as it was.
+ * parents[batch][k] on the device, batch < 2^16, k <= 64; where a parent is < 0 or >= src_beams the row is left as it was.
  * In place (dst == src, same layout): rows are read and written as if all were read first, a row that stays
  * is not touched, rows k.. of an item stay.  Otherwise src and dst must not overlap.  The states of a call must
  * not share bytes with each other.
@@ -355,7 +355,7 @@ int radx_hip_beam_reorder(const radx_hip_beam_state* states, uint32_t n_states, 
  *   out[b][j][t] = tokens[t][b][p(t)],   p(L - 1) = j,   p(t - 1) = parents[t][b][p(t)]
  *
  * where a parent < 0 or >= k stands for the same place.  out[b][j] begins at out + (b * k + j) * out_stride;
- * elements from L on are left as they were.  k <= 128, total_steps < 2^24.
+ * elements from L on are left as they were.  batch < 2^16, k <= 128, total_steps < 2^24.
  */
 int radx_hip_beam_backtrace(const int32_t* tokens, const int32_t* parents, const int32_t* steps, uint32_t total_steps, uint32_t batch,
                             uint32_t k, int32_t* out, uint64_t out_stride, void* stream);

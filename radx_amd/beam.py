@@ -11,28 +11,46 @@ import ctypes
 import functools
 
 from . import capi
-from .sorter import _ptr, _stream
 
-_DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
-_FLAGS = ("torch.bool", "torch.uint8")
+
+def _torch():
+    """torch, with the types these calls take; looked up once."""
+    global _torch
+    import torch
+
+    class names:
+        f32, i32 = torch.float32, torch.int32
+        logits = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+        flags = (torch.bool, torch.uint8)
+        empty, raw_stream = torch.empty, torch._C._cuda_getCurrentRawStream
+    _torch = lambda: names  # noqa: E731
+    return names
+
+
+def _stream(stream, index):
+    """The handle of a stream, by default the device's current one."""
+    return getattr(stream, "cuda_stream", stream) if stream is not None else _torch().raw_stream(index)
 
 
 def _on(t, name, index):
-    if not t.is_cuda:
+    at = t.get_device()
+    if at < 0:
         raise ValueError("%s must be a device tensor" % name)
-    if t.device.index != index:
-        raise ValueError("%s is on %s, expected cuda:%d" % (name, t.device, index))
+    if at != index:
+        raise ValueError("%s is on cuda:%d, expected cuda:%d" % (name, at, index))
 
 
 def _plain(t, dtypes, shape, name, index):
-    """A contiguous tensor of this device, one of these dtypes and this shape."""
-    _on(t, name, index)
-    if str(t.dtype) not in dtypes:
-        raise ValueError("%s must be %s, got %s" % (name, " or ".join(dtypes), t.dtype))
+    """A contiguous tensor of this device, one of these dtypes and this shape; its address."""
+    if t.get_device() != index or index < 0:
+        _on(t, name, index)
+    if t.dtype not in dtypes:
+        raise ValueError("%s must be %s, got %s" % (name, " or ".join(map(str, dtypes)), t.dtype))
     if t.shape != shape:
         raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
     if not t.is_contiguous():
         raise ValueError("%s must be contiguous" % name)
+    return t.data_ptr()
 
 
 class BeamSelector:
@@ -65,69 +83,80 @@ class BeamSelector:
         v & 31 of word v >> 5 admits token v.  finished: bool or uint8 [batch, beams]; such a beam offers end_token
         at its own score.  Equal scores go to the lower beam, the larger logit, the lower token; places that are
         left over get -inf, -1, -1.  out: the tensors to write, as returned."""
-        import torch
-        dev = self.device
-        _on(logits, "logits", dev)
-        dtype = _DTYPES.get(str(logits.dtype))
+        T, dev = _torch(), self.device
+        shape = cum.shape
+        if len(shape) != 2:
+            raise ValueError("cum must be [batch, beams]")
+        batch, beams = shape
+        cum_at = _plain(cum, (T.f32,), shape, "cum", dev)
+        rows = batch * beams
+        if logits.get_device() != dev:
+            _on(logits, "logits", dev)
+        dtype = T.logits.get(logits.dtype)
         if dtype is None:
             raise ValueError("logits must be float32, bfloat16 or float16, got %s" % logits.dtype)
-        if cum.dim() != 2:
-            raise ValueError("cum must be [batch, beams]")
-        batch, beams = cum.shape
-        _plain(cum, ("torch.float32",), cum.shape, "cum", dev)
-        rows, vocab = batch * beams, logits.shape[-1]
-        if logits.dim() == 3 and tuple(logits.shape[:2]) == (batch, beams):
-            stride = logits.stride(1) if beams > 1 else logits.stride(0)
-            if batch > 1 and logits.stride(0) != beams * stride:
+        has, strides = logits.shape, logits.stride()
+        vocab = has[-1]
+        if len(has) == 2 and has[0] == rows:
+            stride = strides[0]
+        elif len(has) == 3 and has[0] == batch and has[1] == beams:
+            stride = strides[1] if beams > 1 else strides[0]
+            if batch > 1 and strides[0] != beams * stride:
                 raise ValueError("logits' rows must be a fixed distance apart")
-        elif logits.dim() == 2 and logits.shape[0] == rows:
-            stride = logits.stride(0)
         else:
-            raise ValueError("logits must be [batch * beams, vocab] or [batch, beams, vocab], got %s for cum %s" % (tuple(logits.shape), (batch, beams)))
-        if vocab > 1 and logits.stride(-1) != 1:
+            raise ValueError("logits must be [batch * beams, vocab] or [batch, beams, vocab], got %s for cum %s" % (tuple(has), (batch, beams)))
+        if strides[-1] != 1 and vocab > 1:
             raise ValueError("the elements of a row of logits must be adjacent")
         if rows <= 1:
             stride = vocab
-        a = capi.BeamSelectArgs()
+        allowed_at = allowed_stride = 0
         if allowed is not None:
             _on(allowed, "allowed", dev)
             words = (vocab + 31) // 32
-            if allowed.dtype != torch.int32 or allowed.dim() != 2 or allowed.shape[0] not in (1, rows) or allowed.shape[1] != words \
+            if allowed.dtype != T.i32 or allowed.dim() != 2 or allowed.shape[0] not in (1, rows) or allowed.shape[1] != words \
                     or (words > 1 and allowed.stride(1) != 1):
                 raise ValueError("allowed must be int32 [batch * beams or 1, ceil(vocab / 32)] with adjacent words")
-            a.allowed = allowed.data_ptr()
-            a.allowed_stride = allowed.stride(0) if allowed.shape[0] > 1 else 0
-        if (finished is None) != (end_token is None):
-            raise ValueError("finished and end_token go together")
-        if finished is not None:
-            _plain(finished, _FLAGS, cum.shape, "finished", dev)
-            a.finished = finished.data_ptr()
-            a.end_token = int(end_token)
+            allowed_at = allowed.data_ptr()
+            allowed_stride = allowed.stride(0) if allowed.shape[0] > 1 else 0
+        finished_at = ended_at = end = 0
+        if finished is not None or end_token is not None:
+            if finished is None or end_token is None:
+                raise ValueError("finished and end_token go together")
+            finished_at = _plain(finished, T.flags, shape, "finished", dev)
+            end = int(end_token)
+            if not 0 <= end < vocab:
+                raise ValueError("end_token %d is outside the vocabulary" % end)
+        if not 1 <= k <= capi.BEAM_MAX_K:
+            raise ValueError("k must be 1..%d, got %d" % (capi.BEAM_MAX_K, k))
+        size = (batch, k)
         if out is None:
             where = cum.device
-            scores = torch.empty((batch, k), dtype=torch.float32, device=where)
-            both = torch.empty((2, batch, k), dtype=torch.int32, device=where)
-            out = (scores, both[0], both[1])
-            if finished is not None:
-                out += (torch.empty((batch, k), dtype=finished.dtype, device=where),)
+            scores = T.empty(size, dtype=T.f32, device=where)
+            parents = T.empty(size, dtype=T.i32, device=where)
+            tokens = T.empty(size, dtype=T.i32, device=where)
+            out = (scores, parents, tokens)
+            at = (scores.data_ptr(), parents.data_ptr(), tokens.data_ptr())
+            if finished_at:
+                ended = T.empty(size, dtype=finished.dtype, device=where)
+                out += (ended,)
+                ended_at = ended.data_ptr()
         else:
             out = tuple(out)
             if len(out) != (3 if finished is None else 4):
                 raise ValueError("out must hold scores, parents, tokens%s" % ("" if finished is None else " and finished flags"))
-            for t, dtypes, name in zip(out, (("torch.float32",), ("torch.int32",), ("torch.int32",), _FLAGS),
-                                       ("out scores", "out parents", "out tokens", "out finished")):
-                _plain(t, dtypes, (batch, k), name, dev)
-        a.logits, a.row_stride, a.cum = logits.data_ptr(), stride, cum.data_ptr()
-        a.scores, a.parents, a.tokens = out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr()
-        if finished is not None:
-            a.out_finished = out[3].data_ptr()
-        a.batch, a.beams, a.vocab, a.k = batch, beams, vocab, k
-        a.dtype, a.normalize = dtype, 1 if normalize else 0
-        capi.check(capi.lib.radx_hip_beam_select(self._h, ctypes.byref(a), _stream(stream, dev)))
+            at = (_plain(out[0], (T.f32,), size, "out scores", dev), _plain(out[1], (T.i32,), size, "out parents", dev),
+                  _plain(out[2], (T.i32,), size, "out tokens", dev))
+            if finished_at:
+                ended_at = _plain(out[3], T.flags, size, "out finished", dev)
+        args = capi.BEAM_SELECT_ARGS.pack(logits.data_ptr(), stride, cum_at, allowed_at, allowed_stride, finished_at, *at, ended_at,
+                                          batch, beams, vocab, k, dtype, 1 if normalize else 0, end)
+        code = capi.lib.radx_hip_beam_select(self._h, args, _stream(stream, dev))
+        if code:
+            capi.check(code)
         return out
 
 
-@functools.lru_cache(maxsize=1024)
+@functools.lru_cache(maxsize=4096)
 def _pieces(shape, src_strides, dst_strides, size, row_dim, length_dim):
     """The rows of a layout as radx_hip_beam_state counts them, strides in bytes:
     (src_row, dst_row, src_outer, dst_outer, outer, unit_bytes, units)."""
@@ -155,6 +184,26 @@ def _pieces(shape, src_strides, dst_strides, size, row_dim, length_dim):
             (outer[0][0], outer[1][0]), run, 1 if units is None else units)
 
 
+@functools.lru_cache(maxsize=4096)
+def _layout(shape, src_strides, dst_strides, size, row_dim, length_dim, batch):
+    """(rows of a batch item, the packed radx_hip_beam_state behind its two addresses) of one state."""
+    dim = len(shape)
+    row = row_dim + dim if row_dim < 0 else row_dim
+    if not 0 <= row < dim:
+        raise ValueError("a state has no dimension %d" % row_dim)
+    if shape[row] % batch:
+        raise ValueError("dimension %d of a state has %d rows, which is not the same number for each of %d items" % (row_dim, shape[row], batch))
+    length = None
+    if length_dim is not None:
+        length = length_dim + dim if length_dim < 0 else length_dim
+        if not 0 <= length < dim or length == row:
+            raise ValueError("length_dim must be a dimension of every state, and not its rows'")
+    if 0 in shape:
+        return shape[row] // batch, None
+    src_row, dst_row, src_outer, dst_outer, outer, unit, units = _pieces(shape, src_strides, dst_strides, size, row, length)
+    return shape[row] // batch, capi.BEAM_STATE.pack(0, 0, src_row, dst_row, *src_outer, *dst_outer, unit, units, *outer)[16:]
+
+
 def beam_reorder(states, parents, into=None, lengths=None, length_dim=None, row_dim=0, stream=None):
     """Moves the survivors' states to their places, all of them in one launch: with parents int32 [batch, k] (k <= 64)
     and `beams` rows an item in dimension row_dim of every state,
@@ -166,52 +215,53 @@ def beam_reorder(states, parents, into=None, lengths=None, length_dim=None, row_
     pieces); they must not share memory with each other.  into: as many tensors that get the rows instead (b * k + j),
     apart from the states.  lengths: int32 [batch]; of dimension length_dim only the first lengths[b] positions
     move, what lies behind is neither read nor written."""
-    states = [states] if hasattr(states, "data_ptr") else list(states)
-    into_list = None if into is None else [into] if hasattr(into, "data_ptr") else list(into)
-    if parents.dim() != 2:
+    states = (states,) if hasattr(states, "data_ptr") else states
+    if into is not None:
+        into = (into,) if hasattr(into, "data_ptr") else into
+        if len(into) != len(states):
+            raise ValueError("into must hold one tensor for each state")
+    T = _torch()
+    shape = parents.shape
+    if len(shape) != 2:
         raise ValueError("parents must be [batch, k]")
-    batch, k = parents.shape
-    dev = parents.device.index
-    _plain(parents, ("torch.int32",), parents.shape, "parents", dev)
-    if (lengths is None) != (length_dim is None):
-        raise ValueError("lengths and length_dim go together")
-    if lengths is not None:
-        _plain(lengths, ("torch.int32",), (batch,), "lengths", dev)
-    if into_list is not None and len(into_list) != len(states):
-        raise ValueError("into must hold one tensor for each state")
-    if not states or batch == 0 or k == 0:
+    batch, k = shape
+    dev = parents.get_device()
+    parents_at = _plain(parents, (T.i32,), shape, "parents", dev)
+    lengths_at = None
+    if lengths is not None or length_dim is not None:
+        if lengths is None or length_dim is None:
+            raise ValueError("lengths and length_dim go together")
+        lengths_at = _plain(lengths, (T.i32,), (batch,), "lengths", dev)
+    if batch == 0 or k == 0:
         return
-    table = (capi.BeamState * len(states))()
-    beams = None
+    table, beams, address = [], None, capi.ADDRESSES.pack
     for i, s in enumerate(states):
-        d = s if into_list is None else into_list[i]
-        _on(s, "a state", dev)
-        dim = s.dim()
-        row = row_dim + dim if row_dim < 0 else row_dim
-        if not 0 <= row < dim:
-            raise ValueError("a state has no dimension %d" % row_dim)
-        if s.shape[row] % batch or (beams is not None and s.shape[row] != beams * batch):
-            raise ValueError("dimension %d of a state has %d rows, which is not the same number for each of %d items" % (row_dim, s.shape[row], batch))
-        beams = s.shape[row] // batch
-        length = None
-        if length_dim is not None:
-            length = length_dim + dim if length_dim < 0 else length_dim
-            if not 0 <= length < dim or length == row:
-                raise ValueError("length_dim must be a dimension of every state, and not its rows'")
-        if d is not s:
+        if s.get_device() != dev:
+            _on(s, "a state", dev)
+        has, strides = s.shape, s.stride()
+        d, d_strides = s, strides
+        if into is not None:
+            d = into[i]
             _on(d, "into", dev)
-            if d.dtype != s.dtype or d.dim() != dim or d.shape[row] != batch * k or d.shape[:row] != s.shape[:row] or d.shape[row + 1:] != s.shape[row + 1:]:
+            row = row_dim + len(has) if row_dim < 0 else row_dim
+            want = tuple(batch * k if n == row else size for n, size in enumerate(has))
+            if d.dtype != s.dtype or d.shape != want:
                 raise ValueError("into must have the states' dtypes and shapes, with batch * k rows")
-        if s.numel() == 0:
-            continue
-        t = table[i]
-        (t.src_row, t.dst_row, (t.src_outer[0], t.src_outer[1]), (t.dst_outer[0], t.dst_outer[1]), (t.outer[0], t.outer[1]),
-         t.unit_bytes, t.units) = _pieces(s.shape, s.stride(), d.stride(), s.element_size(), row, length)
-        t.src, t.dst = s.data_ptr(), d.data_ptr()
-    if not beams:
+            d_strides = d.stride()
+        rows, packed = _layout(has, strides, d_strides, s.element_size(), row_dim, length_dim, batch)
+        if rows != beams:
+            if beams is not None:
+                raise ValueError("the states have different numbers of rows")
+            beams = rows
+        if packed is not None:
+            table.append(address(s.data_ptr(), d.data_ptr()))
+            table.append(packed)
+    if not table or not beams:
         return
-    capi.check(capi.lib.radx_hip_beam_reorder(table, len(states), _ptr(parents), _ptr(lengths), batch, beams, beams if into_list is None else k, k,
-                                              _stream(stream, dev)))
+    code = capi.lib.radx_hip_beam_reorder(b"".join(table), len(table) // 2, parents_at, lengths_at, batch, beams, beams if into is None else k, k,
+                                          _stream(stream, dev))
+    if code:
+        capi.check(code)
 
 
 def beam_backtrace(tokens, parents, steps=None, out=None, stream=None):
@@ -219,25 +269,28 @@ def beam_backtrace(tokens, parents, steps=None, out=None, stream=None):
     [T, batch, k]: out[b, j, t] is the token of step t on the way to place j of step L - 1, with L = steps[b] (int32
     [batch]; None: T).  A parent < 0 or >= k stands for the same place.  Elements from L on are left as they
     were (-1 where `out` is not given)."""
-    if tokens.dim() != 3:
+    T = _torch()
+    shape = tokens.shape
+    if len(shape) != 3:
         raise ValueError("tokens must be [steps, batch, k]")
-    total, batch, k = tokens.shape
-    import torch
-    dev = tokens.device.index
-    _plain(tokens, ("torch.int32",), tokens.shape, "tokens", dev)
-    _plain(parents, ("torch.int32",), tokens.shape, "parents", dev)
-    if steps is not None:
-        _plain(steps, ("torch.int32",), (batch,), "steps", dev)
+    total, batch, k = shape
+    dev = tokens.get_device()
+    tokens_at = _plain(tokens, (T.i32,), shape, "tokens", dev)
+    parents_at = _plain(parents, (T.i32,), shape, "parents", dev)
+    steps_at = None if steps is None else _plain(steps, (T.i32,), (batch,), "steps", dev)
     if out is None:
-        out = torch.empty((batch, k, total), dtype=torch.int32, device=tokens.device)
+        out = T.empty((batch, k, total), dtype=T.i32, device=tokens.device)
         if steps is not None:
             out.fill_(-1)
     _on(out, "out", dev)
-    if out.dtype != torch.int32 or tuple(out.shape) != (batch, k, total) or (total > 1 and out.stride(2) != 1) or \
-            (batch > 1 and k > 1 and out.stride(0) != k * out.stride(1)):
+    strides = out.stride()
+    if out.dtype != T.i32 or out.shape != (batch, k, total) or (total > 1 and strides[2] != 1) or \
+            (batch > 1 and k > 1 and strides[0] != k * strides[1]):
         raise ValueError("out must be int32 [batch, k, steps], its sequences contiguous and a fixed distance apart")
     if total == 0 or batch == 0 or k == 0:
         return out
-    stride = out.stride(1) if k > 1 else out.stride(0) if batch > 1 else total
-    capi.check(capi.lib.radx_hip_beam_backtrace(_ptr(tokens), _ptr(parents), _ptr(steps), total, batch, k, _ptr(out), stride, _stream(stream, dev)))
+    stride = strides[1] if k > 1 else strides[0] if batch > 1 else total
+    code = capi.lib.radx_hip_beam_backtrace(tokens_at, parents_at, steps_at, total, batch, k, out.data_ptr(), stride, _stream(stream, dev))
+    if code:
+        capi.check(code)
     return out

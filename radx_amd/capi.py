@@ -6,6 +6,7 @@ loudly when it is missing.
 """
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libradx_hip.so")
@@ -15,20 +16,13 @@ _u64p = ctypes.POINTER(ctypes.c_uint64)
 _vp = ctypes.c_void_p
 
 
-class BeamSelectArgs(ctypes.Structure):
-    """radx_hip_beam_select_args."""
-    _fields_ = [("logits", _vp), ("row_stride", ctypes.c_uint64), ("cum", _vp), ("allowed", _vp), ("allowed_stride", ctypes.c_uint64),
-                ("finished", _vp), ("scores", _vp), ("parents", _vp), ("tokens", _vp), ("out_finished", _vp),
-                ("batch", ctypes.c_uint32), ("beams", ctypes.c_uint32), ("vocab", ctypes.c_uint32), ("k", ctypes.c_uint32),
-                ("dtype", ctypes.c_int32), ("normalize", ctypes.c_int32), ("end_token", ctypes.c_int32)]
-
-
-class BeamState(ctypes.Structure):
-    """radx_hip_beam_state."""
-    _fields_ = [("src", _vp), ("dst", _vp), ("src_row", ctypes.c_uint64), ("dst_row", ctypes.c_uint64), ("src_outer", ctypes.c_uint64 * 2),
-                ("dst_outer", ctypes.c_uint64 * 2), ("unit_bytes", ctypes.c_uint64), ("units", ctypes.c_uint64),
-                ("outer", ctypes.c_uint32 * 2)]
-
+# radx_hip_beam_select_args and radx_hip_beam_state as struct formats: packing one is several times faster than
+# filling a ctypes.Structure field by field, and these calls are made once a decoded token.
+BEAM_SELECT_ARGS = struct.Struct("=QQQQQQQQQQIIIIiiixxxx")  # logits row_stride cum allowed allowed_stride finished scores
+#                                                           parents tokens out_finished batch beams vocab k dtype normalize end_token
+BEAM_STATE = struct.Struct("=QQQQQQQQQQII")  # src dst src_row dst_row src_outer[2] dst_outer[2] unit_bytes units outer[2]
+ADDRESSES = struct.Struct("=QQ")
+BEAM_MAX_K = 128  # RADX_HIP_BEAM_MAX_K
 
 # Every symbol include/radx_hip.h declares, with its ctypes signature.
 SIGNATURES = {
@@ -65,8 +59,8 @@ SIGNATURES = {
     "radx_hip_beam_scratch_bytes": (ctypes.c_size_t, [ctypes.c_uint32] * 4),
     "radx_hip_beam_create": (ctypes.c_int, [ctypes.c_int] + [ctypes.c_uint32] * 4 + [ctypes.POINTER(_vp)]),
     "radx_hip_beam_destroy": (ctypes.c_int, [_vp]),
-    "radx_hip_beam_select": (ctypes.c_int, [_vp, ctypes.POINTER(BeamSelectArgs), _vp]),
-    "radx_hip_beam_reorder": (ctypes.c_int, [ctypes.POINTER(BeamState), ctypes.c_uint32, _vp, _vp] + [ctypes.c_uint32] * 4 + [_vp]),
+    "radx_hip_beam_select": (ctypes.c_int, [_vp, _vp, _vp]),
+    "radx_hip_beam_reorder": (ctypes.c_int, [_vp, ctypes.c_uint32, _vp, _vp] + [ctypes.c_uint32] * 4 + [_vp]),
     "radx_hip_beam_backtrace": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, _vp, ctypes.c_uint64, _vp]),
     "radx_hip_generate_u32": (ctypes.c_int, [_vp, ctypes.c_uint64, ctypes.c_uint32, _vp]),
     "radx_hip_generate_u64": (ctypes.c_int, [_vp, _vp, ctypes.c_uint64, ctypes.c_uint32, _vp]),

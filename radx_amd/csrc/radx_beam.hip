@@ -769,21 +769,105 @@ struct BacktraceArgs {
     int32_t* out;          // [batch][k][out_stride]
     int64_t out_stride;
     uint32_t total, batch, k;
+    uint32_t segments, segment;  // workgroups an item gets, and the steps that each writes
 };
 
-__global__ __launch_bounds__(kThreads) void beam_backtrace_kernel(BacktraceArgs a) {
-    const uint32_t at = blockIdx.x * kThreads + threadIdx.x;
-    if (at >= a.batch * a.k) return;
-    const uint32_t item = at / a.k;
-    uint32_t place = at - item * a.k;
+// A step's parents are a map of k places, and maps join in any grouping: a workgroup keeps a window of steps in
+// LDS (a byte a place), its groups of threads each walk a chunk of it, a scan over the chunks' maps
+// tells where every chunk is entered from, and a second walk writes down the way.  A window's chain of n
+// dependent look-ups becomes one of 2 n / groups + log2(groups), all of them in LDS.  A segment's workgroup
+// walks through everything behind it first, which needs no traffic between workgroups.
+constexpr uint32_t kTraceThreads = 1024;
+constexpr uint32_t kWindow = 32768;  // places in LDS at once
+
+__global__ __launch_bounds__(kTraceThreads) void beam_backtrace_kernel(BacktraceArgs a) {
+    __shared__ __attribute__((aligned(16))) uint8_t parent_of[kWindow];
+    __shared__ __attribute__((aligned(16))) uint8_t way[kWindow];
+    __shared__ uint8_t maps[2][kTraceThreads];
+    __shared__ uint8_t entry[2][kMaxK];
+    // an XCD's workgroups (every eighth) take neighbouring items with all their segments: a line of a step's
+    // row holds several items, and a segment reads what the later ones read, so its L2 serves them all
+    const uint32_t xcd = blockIdx.x & 7u, share = gridDim.x >> 3, more = gridDim.x & 7u;
+    const uint32_t place = xcd * share + min(xcd, more) + (blockIdx.x >> 3);
+    const uint32_t item = place / a.segments, k = a.k;
+    uint32_t wide = 1;
+    while (wide < k) wide <<= 1;
+    const uint32_t groups = kTraceThreads / wide, group = threadIdx.x / wide, j = threadIdx.x & (wide - 1u);
     uint32_t ends = a.total;
     if (a.steps) ends = min(a.total, static_cast<uint32_t>(max(0, a.steps[item])));
-    int32_t* out = a.out + static_cast<int64_t>(at) * a.out_stride;
-    for (uint32_t t = ends; t-- > 0;) {
-        const size_t from = (static_cast<size_t>(t) * a.batch + item) * a.k + place;
-        out[t] = a.tokens[from];
-        const uint32_t p = static_cast<uint32_t>(a.parents[from]);
-        if (p < a.k) place = p;
+    const uint32_t s0 = (place - item * a.segments) * a.segment, s1 = min(ends, s0 + a.segment);
+    if (s0 >= ends) return;
+    const uint32_t window = kWindow / k;
+    const size_t step_places = static_cast<size_t>(a.batch) * k;
+    uint32_t turn = 0;
+    if (threadIdx.x < k) entry[0][threadIdx.x] = static_cast<uint8_t>(threadIdx.x);
+    for (uint32_t w1 = ends; w1 > s0;) {
+        const bool own = w1 <= s1;
+        const uint32_t border = own ? s0 : s1;
+        const uint32_t w0 = w1 - border > window ? w1 - window : border, n = w1 - w0;
+        const int32_t* from = a.parents + w0 * step_places + static_cast<size_t>(item) * k;
+        __syncthreads();
+        if ((k & 3u) == 0) {
+            // four places at a time; a step's row is whole fours
+            const uint32_t quads = k >> 2;
+#pragma unroll 4
+            for (uint32_t i = threadIdx.x; i < n * quads; i += kTraceThreads) {
+                const uint32_t t = i / quads, p = (i - t * quads) * 4;
+                const Bytes16 v = *reinterpret_cast<const Bytes16*>(from + t * step_places + p);
+                uint32_t packed = 0;
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) packed |= (v.w[e] < k ? v.w[e] : p + e) << (8 * e);
+                reinterpret_cast<uint32_t*>(parent_of)[i] = packed;
+            }
+        } else {
+#pragma unroll 4
+            for (uint32_t i = threadIdx.x; i < n * k; i += kTraceThreads) {
+                const uint32_t t = i / k, p = i - t * k;
+                const uint32_t v = static_cast<uint32_t>(from[t * step_places + p]);
+                parent_of[i] = static_cast<uint8_t>(v < k ? v : p);
+            }
+        }
+        __syncthreads();
+        const uint32_t chunk = (n + groups - 1) / groups;
+        const uint32_t c0 = min(n, group * chunk), c1 = min(n, c0 + chunk);
+        uint32_t at = j;
+        if (j < k)
+            for (uint32_t t = c1; t-- > c0;) at = parent_of[t * k + at];
+        uint32_t side = 0;
+        maps[0][threadIdx.x] = static_cast<uint8_t>(at);
+        __syncthreads();
+        // maps[group]: from behind the window to before this chunk
+        for (uint32_t d = 1; d < groups; d <<= 1, side ^= 1) {
+            uint32_t v = j;
+            if (j < k) {
+                if (group + d < groups) v = maps[side][(group + d) * wide + j];
+                v = maps[side][group * wide + v];
+            }
+            maps[side ^ 1][threadIdx.x] = static_cast<uint8_t>(v);
+            __syncthreads();
+        }
+        if (j < k) {
+            at = entry[turn][j];
+            if (group == 0) entry[turn ^ 1][j] = maps[side][at];
+            if (own) {
+                if (group + 1 < groups) at = maps[side][(group + 1) * wide + at];
+                for (uint32_t t = c1; t-- > c0;) {
+                    way[t * k + j] = static_cast<uint8_t>(at);
+                    at = parent_of[t * k + at];
+                }
+            }
+        }
+        turn ^= 1;
+        __syncthreads();
+        if (own) {
+            const int32_t* tokens = a.tokens + w0 * step_places + static_cast<size_t>(item) * k;
+            int32_t* out = a.out + static_cast<int64_t>(item) * k * a.out_stride + w0;
+            // sequences are written along their length; the k look-ups of a step hit the same lines
+            for (uint32_t t = threadIdx.x; t < n; t += kTraceThreads)
+#pragma unroll 4
+                for (uint32_t p = 0; p < k; ++p) out[p * a.out_stride + t] = tokens[t * step_places + way[t * k + p]];
+        }
+        w1 = w0;
     }
 }
 
@@ -1036,7 +1120,7 @@ int radx_hip_beam_reorder(const radx_hip_beam_state* states, uint32_t n_states, 
 int radx_hip_beam_backtrace(const int32_t* tokens, const int32_t* parents, const int32_t* steps, uint32_t total_steps, uint32_t batch,
                             uint32_t k, int32_t* out, uint64_t out_stride, void* stream) {
     if (k < 1 || k > kMaxK) return bad_arg("k must be 1..128");
-    if (batch > (1u << 20)) return bad_arg("batch must be at most 2^20");
+    if (batch > 65535) return bad_arg("batch must be < 2^16");
     if (total_steps >= (1u << 24)) return bad_arg("total_steps must be < 2^24");
     if (batch == 0 || total_steps == 0) return 0;
     if (!tokens || !parents || !out) return bad_arg("NULL buffer");
@@ -1048,9 +1132,14 @@ int radx_hip_beam_backtrace(const int32_t* tokens, const int32_t* parents, const
     if (overlap(out, out_bytes, tokens, in_bytes) || overlap(out, out_bytes, parents, in_bytes) || overlap(out, out_bytes, steps, batch * 4ull))
         return bad_arg("out overlaps an input");
     RADX_ON_DEVICE_OF(out);
-    const BacktraceArgs a{tokens, parents, steps, out, static_cast<int64_t>(out_stride), total_steps, batch, k};
-    hipLaunchKernelGGL(beam_backtrace_kernel, dim3(static_cast<uint32_t>((places + kThreads - 1) / kThreads)), dim3(kThreads), 0,
-                       static_cast<hipStream_t>(stream), a);
+    // a workgroup a CU where the sequences are long enough to be cut
+    const uint64_t most = (static_cast<uint64_t>(total_steps) * k + 4095) / 4096;
+    uint64_t segments = batch >= 256 ? 1 : 256 / batch;
+    if (segments > most) segments = most;
+    const uint32_t segment = static_cast<uint32_t>((total_steps + segments - 1) / segments);
+    const uint32_t cuts = (total_steps + segment - 1) / segment;
+    const BacktraceArgs a{tokens, parents, steps, out, static_cast<int64_t>(out_stride), total_steps, batch, k, cuts, segment};
+    hipLaunchKernelGGL(beam_backtrace_kernel, dim3(cuts * batch), dim3(kTraceThreads), 0, static_cast<hipStream_t>(stream), a);
     RADX_TRY(hipGetLastError());
     return 0;
 }

@@ -17,13 +17,11 @@ def refused(code, text):
 
 
 def select_args(**change):
-    a = capi.BeamSelectArgs()
-    a.logits, a.row_stride, a.cum = BASE, 1000, BASE + (1 << 30)
-    a.scores, a.parents, a.tokens = BASE + (2 << 30), BASE + (3 << 30), BASE + (4 << 30)
-    a.batch, a.beams, a.vocab, a.k, a.dtype, a.normalize = 2, 4, 1000, 8, 1, 1
-    for name, value in change.items():
-        setattr(a, name, value)
-    return a
+    a = dict(logits=BASE, row_stride=1000, cum=BASE + (1 << 30), allowed=None, allowed_stride=0, finished=None, scores=BASE + (2 << 30),
+             parents=BASE + (3 << 30), tokens=BASE + (4 << 30), out_finished=None, batch=2, beams=4, vocab=1000, k=8, dtype=1, normalize=1,
+             end_token=0)
+    a.update(change)
+    return capi.BEAM_SELECT_ARGS.pack(*(value or 0 for value in a.values()))
 
 
 @pytest.mark.parametrize("change,text", [
@@ -42,11 +40,11 @@ def select_args(**change):
     (dict(), "handle is NULL"), (dict(row_stride=0), "handle is NULL"), (dict(allowed=BASE + (5 << 30), allowed_stride=0), "handle is NULL"),
 ])
 def test_select_refuses(change, text):
-    refused(capi.lib.radx_hip_beam_select(None, ctypes.byref(select_args(**change)), None), text)
+    refused(capi.lib.radx_hip_beam_select(None, select_args(**change), None), text)
 
 
 def test_an_empty_batch_is_no_error():
-    assert capi.lib.radx_hip_beam_select(None, ctypes.byref(select_args(batch=0)), None) == 0
+    assert capi.lib.radx_hip_beam_select(None, select_args(batch=0), None) == 0
     assert capi.lib.radx_hip_beam_reorder(None, 0, None, None, 0, 4, 4, 4, None) == 0
     assert capi.lib.radx_hip_beam_backtrace(None, None, None, 0, 2, 4, None, 0, None) == 0
     assert capi.lib.radx_hip_beam_destroy(None) == 0
@@ -62,23 +60,34 @@ def test_create_refuses_limits():
 
 
 def state(**change):
-    s = capi.BeamState()
-    s.src = s.dst = BASE
-    s.src_row = s.dst_row = 4096
-    s.src_outer[0] = s.src_outer[1] = s.dst_outer[0] = s.dst_outer[1] = 0
-    s.outer[0] = s.outer[1] = 1
-    s.unit_bytes, s.units = 64, 64
-    for name, value in change.items():
-        if isinstance(value, tuple):
-            getattr(s, name)[0], getattr(s, name)[1] = value
-        else:
-            setattr(s, name, value)
-    return s
+    s = dict(src=BASE, dst=BASE, src_row=4096, dst_row=4096, src_outer=(0, 0), dst_outer=(0, 0), unit_bytes=64, units=64, outer=(1, 1))
+    s.update(change)
+    flat = []
+    for value in s.values():
+        flat += value if isinstance(value, tuple) else [value or 0]
+    return capi.BEAM_STATE.pack(*flat)
 
 
 def reorder(states, batch=2, src=4, dst=4, k=4, parents=BASE + (1 << 30)):
-    table = (capi.BeamState * max(1, len(states)))(*states)
-    return capi.lib.radx_hip_beam_reorder(table, len(states), parents, None, batch, src, dst, k, None)
+    return capi.lib.radx_hip_beam_reorder(b"".join(states), len(states), parents, None, batch, src, dst, k, None)
+
+
+def test_struct_formats_are_the_headers(tmp_path):
+    """The packed formats are the C structs, field by field."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    fields = ["logits", "row_stride", "cum", "allowed", "allowed_stride", "finished", "scores", "parents", "tokens", "out_finished", "batch",
+              "beams", "vocab", "k", "dtype", "normalize", "end_token"]
+    state_fields = ["src", "dst", "src_row", "dst_row", "src_outer", "dst_outer", "unit_bytes", "units", "outer"]
+    lines = ["offsetof(radx_hip_beam_select_args, %s)" % f for f in fields] + ["sizeof(radx_hip_beam_select_args)"]
+    lines += ["offsetof(radx_hip_beam_state, %s)" % f for f in state_fields] + ["sizeof(radx_hip_beam_state)"]
+    src = tmp_path / "o.c"
+    src.write_text('#include <stdio.h>\n#include "radx_hip.h"\nint main(void) {' + "".join('printf("%%zu\\n", %s);' % e for e in lines) + "return 0; }\n")
+    subprocess.run(["gcc", "-I" + os.path.join(root, "include"), "-o", str(tmp_path / "o"), str(src)], check=True, timeout=60)
+    got = [int(v) for v in subprocess.run([str(tmp_path / "o")], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [8 * i for i in range(10)] + [80 + 4 * i for i in range(7)] + [capi.BEAM_SELECT_ARGS.size] + \
+        [0, 8, 16, 24, 32, 48, 64, 72, 80] + [capi.BEAM_STATE.size]
 
 
 @pytest.mark.parametrize("change,text", [
@@ -112,7 +121,7 @@ def test_backtrace_refuses():
         return capi.lib.radx_hip_beam_backtrace(tokens, parents, steps, total, batch, k, out, stride, None)
     refused(call(k=0), "k must")
     refused(call(k=129), "k must")
-    refused(call(batch=(1 << 20) + 1), "batch")
+    refused(call(batch=65536), "batch")
     refused(call(total=1 << 24), "total_steps")
     refused(call(tokens=None), "NULL")
     refused(call(parents=None), "NULL")

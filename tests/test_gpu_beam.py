@@ -401,10 +401,11 @@ def test_select_refuses_tensors(device):
                      ((x, cum, 8), dict(out=(cum, cum)))):
         with pytest.raises(ValueError):
             sel.select(*args, **kw)
-    with pytest.raises(radx_amd.RadxError, match="end_token"):
+    with pytest.raises(ValueError, match="end_token"):
         sel.select(x, cum, 8, finished=flags, end_token=100)
-    with pytest.raises(radx_amd.RadxError, match="k must"):
-        sel.select(x, cum, 0)
+    for k in (0, -1, 129):
+        with pytest.raises(ValueError, match="k must"):
+            sel.select(x, cum, k)
     both = torch.zeros(2, 4, dtype=torch.int32, device=device)
     with pytest.raises(radx_amd.RadxError, match="overlap"):
         sel.select(x, cum, 4, out=(cum, both, torch.zeros_like(both)))
