@@ -22,7 +22,7 @@ def _torch():
         f32, i32 = torch.float32, torch.int32
         logits = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
         flags = (torch.bool, torch.uint8)
-        empty, raw_stream = torch.empty, torch._C._cuda_getCurrentRawStream
+        empty, empty_like, raw_stream = torch.empty, torch.empty_like, torch._C._cuda_getCurrentRawStream
     _torch = lambda: names  # noqa: E731
     return names
 
@@ -130,14 +130,13 @@ class BeamSelector:
             raise ValueError("k must be 1..%d, got %d" % (capi.BEAM_MAX_K, k))
         size = (batch, k)
         if out is None:
-            where = cum.device
-            scores = T.empty(size, dtype=T.f32, device=where)
-            parents = T.empty(size, dtype=T.i32, device=where)
-            tokens = T.empty(size, dtype=T.i32, device=where)
+            scores = cum.new_empty(size)  # the cheapest of torch's ways
+            parents = cum.new_empty(size, dtype=T.i32)
+            tokens = T.empty_like(parents)
             out = (scores, parents, tokens)
             at = (scores.data_ptr(), parents.data_ptr(), tokens.data_ptr())
             if finished_at:
-                ended = T.empty(size, dtype=finished.dtype, device=where)
+                ended = finished.new_empty(size)
                 out += (ended,)
                 ended_at = ended.data_ptr()
         else:

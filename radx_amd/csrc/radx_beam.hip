@@ -70,10 +70,35 @@ __device__ __forceinline__ float wave_max(float v) {
 __device__ __forceinline__ uint32_t lanes_before(uint64_t mask) {
     return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0u));
 }
+// The sum of a wave's values, in every lane.
 __device__ __forceinline__ double wave_sum(double v) {
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+#define RADX_DPP_SUM(ctrl, rows)                                                                                     \
+    {                                                                                                                \
+        const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v));                                           \
+        const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(u), ctrl, rows, 0xf, false));         \
+        const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), ctrl, rows, 0xf, false));   \
+        v += __longlong_as_double(static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo));                       \
+    }
+    RADX_DPP_SUM(0x111, 0xf)  // row_shr:1
+    RADX_DPP_SUM(0x112, 0xf)
+    RADX_DPP_SUM(0x114, 0xf)
+    RADX_DPP_SUM(0x118, 0xf)
+    RADX_DPP_SUM(0x142, 0xa)  // row_bcast:15 into rows 1 and 3
+    RADX_DPP_SUM(0x143, 0xc)  // row_bcast:31 into rows 2 and 3
+#undef RADX_DPP_SUM
+    const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v));
+    const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(u), 63));
+    const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(u >> 32), 63));
+    return __longlong_as_double(static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo));
 }
+// A value that all lanes of a wave have, as the scalar that it is.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v))); }
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(uniform(__float_as_uint(v))); }
+__device__ __forceinline__ uint64_t uniform(uint64_t v) {
+    return static_cast<uint64_t>(uniform(static_cast<uint32_t>(v >> 32))) << 32 | uniform(static_cast<uint32_t>(v));
+}
+// i / d by m = ceil(2^32 / d), for i * d < 2^32
+__device__ __forceinline__ uint32_t divided(uint32_t i, uint32_t d, uint32_t m) { return d == 1 ? i : __umulhi(i, m); }
 
 // Elements of one 16-byte vector as floats; tail(): the first n elements at p, -inf behind them.
 template <typename T> struct Vec;
@@ -162,18 +187,23 @@ __device__ __forceinline__ uint32_t end_of_bin(uint32_t bin) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// selection, first kernel: one workgroup takes a slice of one row
+// selection
 // ---------------------------------------------------------------------------------------------
-// score(row, token) = cum[row] + ((x - M) - log sum exp(x - M)): within a row the order of the scores
+// One workgroup takes a slice of one row, and one the slices of an item.  score(row, token) = cum[row] + ((x - M) - log sum exp(x - M)): within a row the order of the scores
 // is the order of the logits, so a slice can be searched for its own k best before M and the sum
 // are known.  A slice leaves its maximum, its sum of exponentials relative to that maximum, and its
 // k best logits.
 struct SliceInfo {
-    double sum;      // of exp(x - max)
+    uint64_t sum;    // of exp(x - max): a double's bits
     uint64_t head;   // the slice's best entry (0: none)
-    float max;
-    uint32_t pad;
+    uint64_t max;    // a float's bits
 };
+
+// What slices leave for the join, where the join may be a workgroup of the same launch on another XCD: words
+// that go through to where every XCD sees them, and are fetched from there.  A fence for all of
+// memory would write back and drop the L2 for every workgroup (16 x 8 x 65536: 36 us instead of 15).
+__device__ __forceinline__ void publish(uint64_t* p, uint64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ uint64_t published(const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 struct SelectArgs {
     const void* logits;
@@ -186,8 +216,10 @@ struct SelectArgs {
     int normalize;
     uint32_t beams, vocab, k;
     uint32_t slices, tiles_per_slice;
+    uint32_t k_inverse, slices_inverse;  // ceil(2^32 / d), for divided()
     SliceInfo* info;            // [row][slice]
     uint64_t* best;             // [row][slice][k]: ordered logit, then ~token; 0: none
+    uint32_t* arrived;          // [batch]: slices of an item that are done; 0 between calls
     float* scores;
     int32_t* parents;
     int32_t* tokens;
@@ -196,6 +228,286 @@ struct SelectArgs {
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
+// ---------------------------------------------------------------------------------------------
+// selection, the join: one workgroup takes one batch item
+// ---------------------------------------------------------------------------------------------
+// The rows' maxima and sums are joined from their slices, every slice's entries get their scores in
+// 64 bits, and the k best come out in the order (score down, beam up, logit down, token up).
+// Within a beam that is the slices' own order.
+constexpr uint32_t kMergeStage = 512;
+constexpr uint32_t kMergeThreads = 1024;  // of the join as a kernel of its own
+constexpr uint32_t kHeldJoined = 2;       // entries a thread holds in the join inside the slices' kernel
+constexpr uint32_t kHeldMost = 16;        // and in the one of its own
+
+struct Entry {
+    uint64_t score;  // ordered64
+    uint64_t rest;   // beam, ~ordered logit, token: smaller is better
+};
+__device__ __forceinline__ bool better(const Entry& p, const Entry& q) {
+    return p.score > q.score || (p.score == q.score && p.rest < q.rest);
+}
+
+struct RowBase {
+    double top, log_sum, cum;
+};
+
+__device__ __forceinline__ double score_of(const RowBase& r, uint64_t key) {
+    return r.cum + ((static_cast<double>(from_ordered(static_cast<uint32_t>(key >> 32))) - r.top) - r.log_sum);
+}
+
+// A float not below v.
+__device__ __forceinline__ float rounded_up(double v) {
+    const float f = static_cast<float>(v);
+    return static_cast<double>(f) < v ? from_ordered(ordered(f) + 1u) : f;
+}
+
+__device__ __forceinline__ Entry entry_of(const RowBase& r, uint32_t beam, uint64_t key) {
+    const uint32_t o = static_cast<uint32_t>(key >> 32), token = ~static_cast<uint32_t>(key);
+    return Entry{ordered64(score_of(r, key)), static_cast<uint64_t>(beam) << 56 | static_cast<uint64_t>(~o) << 24 | token};
+}
+// The k best of from[0..n_from) and stage[0..n) into to[], sorted: an entry's place is the number of better ones.
+// Arrays have room for eight entries behind their last, which are made the worst there are.
+template <uint32_t THREADS>
+__device__ __forceinline__ uint32_t prune(Entry* from, uint32_t n_from, Entry* stage, uint32_t n, Entry* to, uint32_t k) {
+    const uint32_t all = n_from + n;
+    if (threadIdx.x < 8) {
+        from[n_from + threadIdx.x] = Entry{0, 0};
+        stage[n + threadIdx.x] = Entry{0, 0};
+    }
+    __syncthreads();
+    // lanes an entry gets: up to eight, as long as each has eight entries to compare with
+    uint32_t parts = 1;
+    while (parts < 8 && parts * 8 < all && 2 * parts * all <= THREADS) parts <<= 1;
+    const uint32_t part = threadIdx.x & (parts - 1u);
+    auto count = [&](const Entry* list, uint32_t size, const Entry& e) {
+        uint32_t above = 0;
+        for (uint32_t j = part * 8; j < size; j += parts * 8) {
+            Entry other[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) other[i] = list[j + i];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) above += better(other[i], e);
+        }
+        return above;
+    };
+    for (uint32_t i = threadIdx.x / parts; i < all; i += THREADS / parts) {
+        const Entry e = i < n_from ? from[i] : stage[i - n_from];
+        uint32_t above = count(from, n_from, e) + count(stage, n, e);
+        for (uint32_t o = parts >> 1; o; o >>= 1) above += __shfl_xor(above, o);
+        if (above < k) to[above] = e;  // from all of the entry's lanes
+    }
+    __syncthreads();
+    return all < k ? all : k;
+}
+
+// Bins of scores by their distance below the best one, four for every power of two from 2^-44 up.
+__device__ __forceinline__ uint32_t bin_of(double best, double score) {
+    const uint32_t b = __float_as_uint(static_cast<float>(best - score)) >> 21;  // exponent and two bits of the fraction
+    constexpr uint32_t kLow = (127 - 44) * 4;
+    return b <= kLow ? 0 : min(b - kLow, kBins - 1);
+}
+
+__device__ __forceinline__ float max_of(const SliceInfo& s) { return __uint_as_float(static_cast<uint32_t>(published(&s.max))); }
+
+__device__ __forceinline__ double sum_of(const SliceInfo& s) { return __longlong_as_double(static_cast<int64_t>(published(&s.sum))); }
+
+struct MergeLds {
+    uint32_t bins[kBins];
+    Entry kept[2][kMaxK + 8];
+    Entry stage[kMergeStage + 8];
+    RowBase base[kMaxBeams];
+    float wave_best[16];
+    uint32_t staged, looked;
+};
+
+// HELD: every list's entries are held in registers, at most so many a thread.  0: `heads` has room for two words a
+// list, and the lists whose best entry is not among the k best of these are left out.
+template <uint32_t THREADS, uint32_t HELD>
+__device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, MergeLds& lds, uint32_t* heads) {
+    constexpr bool ALL = HELD > 0;
+    RowBase* const base = lds.base;
+    Entry* const stage = lds.stage;
+    uint32_t* const bins = lds.bins;
+    uint32_t& staged = lds.staged;
+    uint32_t& looked = lds.looked;
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t lists = a.beams * a.slices;
+    const SliceInfo* info = a.info + static_cast<size_t>(item) * lists;
+    const uint64_t* best = a.best + static_cast<size_t>(item) * lists * a.k;
+    uint32_t* look = heads + lists;
+
+    uint64_t held[ALL ? HELD : 1];
+    if (ALL) {
+#pragma unroll
+        for (uint32_t r = 0; r < HELD; ++r) held[r] = threadIdx.x + r * THREADS < lists * a.k ? published(&best[threadIdx.x + r * THREADS]) : 0;
+    }
+    if (threadIdx.x == 0) staged = looked = 0;
+    if (threadIdx.x < kBins) bins[threadIdx.x] = 0;
+    __syncthreads();
+    // rows: a group of lanes each, a power of two that covers the slices
+    uint32_t group = 1;
+    while (group < a.slices && group < 64) group <<= 1;
+    const uint32_t first = threadIdx.x & (group - 1u);
+    float most = -INFINITY;  // the best score among this thread's rows, rounded up
+    for (uint32_t beam = threadIdx.x / group; beam < a.beams; beam += THREADS / group) {
+        const uint32_t row = item * a.beams + beam;
+        const float cum = a.cum[row];
+        const bool ended = a.finished && a.finished[row];
+        const SliceInfo* mine = info + beam * a.slices;
+        // the first slice of every lane is fetched whole before any is looked at; most rows have no more
+        const bool some = first < a.slices;
+        const float m0 = some ? max_of(mine[first]) : -INFINITY;
+        const double s0 = some ? sum_of(mine[first]) : 0.0;
+        float m = m0;
+        for (uint32_t s = first + group; s < a.slices; s += group) m = fmaxf(m, max_of(mine[s]));
+        for (uint32_t o = group >> 1; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        auto scaled = [&](float ms, double p) {
+            return ms > -INFINITY || !(p == 0.0) ? p * exp(static_cast<double>(ms) - static_cast<double>(m)) : 0.0;
+        };
+        double sum = scaled(m0, s0);
+        for (uint32_t s = first + group; s < a.slices; s += group) sum += scaled(max_of(mine[s]), sum_of(mine[s]));
+        for (uint32_t o = group >> 1; o; o >>= 1) sum += __shfl_xor(sum, o);
+        // a NaN or +inf among the allowed logits has made the sum a NaN
+        const bool live = !ended && finite(cum) && finite(m) && sum > 0.0 && sum < INFINITY;
+        const RowBase r{a.normalize ? static_cast<double>(m) : 0.0, a.normalize ? log(sum) : 0.0, live ? static_cast<double>(cum) : -INFINITY};
+        if (live) most = fmaxf(most, rounded_up(score_of(r, static_cast<uint64_t>(ordered(m)) << 32)));
+        if (first == 0) {
+            base[beam] = r;
+            if (ended && finite(cum)) {
+                stage[atomicAdd(&staged, 1u)] = Entry{ordered64(cum), static_cast<uint64_t>(beam) << 56 | static_cast<uint32_t>(a.end_token)};
+                most = fmaxf(most, cum);
+            }
+        }
+    }
+    most = wave_max(most);
+    if (lane == 0) lds.wave_best[threadIdx.x >> 6] = most;
+    __syncthreads();
+    for (uint32_t w = 0; w < THREADS / 64; ++w) most = fmaxf(most, lds.wave_best[w]);
+    const double top = static_cast<double>(most);
+
+    const uint32_t ended_beams = staged;
+    uint32_t n_look = lists;
+    uint32_t limit = kBins - 1;  // the bin up to which k lists have their best entry: no other entry is wanted
+    if (HELD == 0 || HELD > 2) {
+        for (uint32_t l = threadIdx.x; l < lists; l += THREADS) {
+            const uint32_t beam = divided(l, a.slices, a.slices_inverse);
+            const uint64_t head = base[beam].cum > -INFINITY ? published(&info[l].head) : 0;
+            const uint32_t bin = head ? bin_of(top, score_of(base[beam], head)) : kBins;
+            if (!ALL) heads[l] = bin;
+            if (bin < kBins) atomicAdd(&bins[bin], 1u);
+        }
+        if (threadIdx.x < ended_beams) atomicAdd(&bins[bin_of(top, from_ordered64(stage[threadIdx.x].score))], 1u);
+        __syncthreads();
+        limit = bin_with(bins, a.k);
+        __syncthreads();
+        if (!ALL)
+            for (uint32_t l = threadIdx.x; l < lists; l += THREADS)
+                if (heads[l] <= limit) look[atomicAdd(&looked, 1u)] = l;
+        if (threadIdx.x < kBins) bins[threadIdx.x] = 0;
+        __syncthreads();
+        if (!ALL) n_look = looked;
+    }
+    // which entries: those among the k best by the same count
+    const uint32_t some = n_look * a.k;
+    auto beam_at = [&](uint32_t i) {
+        const uint32_t which = divided(i, a.k, a.k_inverse);
+        return divided(ALL ? which : look[which], a.slices, a.slices_inverse);
+    };
+    auto key_at = [&](uint32_t i) {
+        const uint32_t which = divided(i, a.k, a.k_inverse);
+        return best[static_cast<size_t>(ALL ? which : look[which]) * a.k + (i - which * a.k)];
+    };
+    auto offered = [&](uint64_t key, uint32_t beam) { return base[beam].cum > -INFINITY && key != 0; };
+    auto count = [&](uint64_t key, uint32_t i) -> uint32_t {
+        if (!key) return kBins;
+        const uint32_t beam = beam_at(i);
+        if (!offered(key, beam)) return kBins;
+        const uint32_t bin = bin_of(top, score_of(base[beam], key));
+        if (bin <= limit) atomicAdd(&bins[bin], 1u);  // most entries are far away, in few bins: their counts would queue
+        return bin;
+    };
+    uint32_t bin_held[ALL ? HELD : 1];
+    if (ALL) {
+#pragma unroll
+        for (uint32_t r = 0; r < HELD; ++r)
+            if (r * THREADS < some) bin_held[r] = count(held[r], threadIdx.x + r * THREADS);
+    } else {
+        for (uint32_t i = threadIdx.x; i < some; i += THREADS) count(key_at(i), i);
+    }
+    if (threadIdx.x < ended_beams) atomicAdd(&bins[bin_of(top, from_ordered64(stage[threadIdx.x].score))], 1u);
+    __syncthreads();
+    const uint32_t upto = min(bin_with(bins, a.k), limit);
+    auto take = [&](uint64_t key, uint32_t beam) {
+        const uint32_t at = atomicAdd(&staged, 1u);
+        if (at < kMergeStage) stage[at] = entry_of(base[beam], beam, key);
+    };
+    if (ALL) {
+#pragma unroll
+        for (uint32_t r = 0; r < HELD; ++r)
+            if (r * THREADS < some && bin_held[r] <= upto) take(held[r], beam_at(threadIdx.x + r * THREADS));
+    } else {
+        for (uint32_t i = threadIdx.x; i < some; i += THREADS) {
+            const uint64_t key = key_at(i);
+            const uint32_t beam = beam_at(i);
+            if (offered(key, beam) && bin_of(top, score_of(base[beam], key)) <= upto) take(key, beam);
+        }
+    }
+    __syncthreads();
+    Entry* kept = lds.kept[0];
+    uint32_t n_kept = 0;
+    if (staged <= kMergeStage) {
+        n_kept = prune<THREADS>(lds.kept[1], 0, stage, staged, kept, a.k);
+    } else {
+        // very many ties: the lists a few at a time
+        n_kept = prune<THREADS>(lds.kept[1], 0, stage, ended_beams, kept, a.k);
+        uint32_t turn = 1;
+        const uint32_t step = kMergeStage / a.k;
+        for (uint32_t l0 = 0; l0 < n_look; l0 += step) {
+            if (threadIdx.x == 0) staged = 0;
+            __syncthreads();
+            const uint32_t now = min(step, n_look - l0) * a.k;
+            for (uint32_t i = threadIdx.x; i < now; i += THREADS) {
+                const uint64_t key = key_at(l0 * a.k + i);
+                const uint32_t beam = beam_at(l0 * a.k + i);
+                if (!offered(key, beam) || bin_of(top, score_of(base[beam], key)) > upto) continue;
+                const Entry e = entry_of(base[beam], beam, key);
+                if (n_kept == a.k && !better(e, kept[a.k - 1])) continue;
+                stage[atomicAdd(&staged, 1u)] = e;
+            }
+            __syncthreads();
+            n_kept = prune<THREADS>(kept, n_kept, stage, staged, lds.kept[turn], a.k);
+            kept = lds.kept[turn];
+            turn ^= 1;
+        }
+    }
+
+    for (uint32_t i = threadIdx.x; i < a.k; i += THREADS) {
+        const size_t at = static_cast<size_t>(item) * a.k + i;
+        float score = -INFINITY;
+        int32_t parent = -1, token = -1;
+        if (i < n_kept) {
+            score = static_cast<float>(from_ordered64(kept[i].score));  // the one rounding of a score
+            parent = static_cast<int32_t>(kept[i].rest >> 56);
+            token = static_cast<int32_t>(kept[i].rest & 0xffffffu);
+        }
+        a.scores[at] = score;
+        a.parents[at] = parent;
+        a.tokens[at] = token;
+        if (a.out_finished)
+            a.out_finished[at] = parent >= 0 && (token == a.end_token || a.finished[item * a.beams + parent]);
+    }
+}
+
+template <uint32_t HELD>
+__global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(SelectArgs a) {
+    extern __shared__ uint32_t heads[];
+    __shared__ __attribute__((aligned(16))) MergeLds lds;
+    merge_item<kMergeThreads, HELD>(a, blockIdx.x, lds, heads);
+}
+
+// ---------------------------------------------------------------------------------------------
+// selection, the slices
+// ---------------------------------------------------------------------------------------------
 // Orders a wave's LDS traffic between its lanes: the wave runs in step and its LDS operations are
 // done in order, so only the compiler has to be held back.
 __device__ __forceinline__ void wave_fence() {
@@ -203,7 +515,8 @@ __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
-constexpr uint32_t kWaveList = 512;  // entries a wave can hold while it looks through a tile
+// Entries a wave can hold while it looks through a tile: 320, one vector of every lane more, and padding.
+constexpr uint32_t kWaveList = 320 + 512 + 64;
 
 // The k-th largest of list[0..n), n >= k; the keys are unique and none is 0.  For lists that grew too long only.
 __device__ __forceinline__ uint64_t kth_key(const uint64_t* list, uint32_t n, uint32_t k) {
@@ -285,13 +598,22 @@ struct TilePart {
     }
 };
 
-// The number of entries in a workgroup's lists that are larger than key.
-__device__ __forceinline__ uint32_t larger(const uint64_t (*lists)[kWaveList], const uint32_t* listed, uint64_t key) {
+// Zeros behind a list, so that it can be read in eights.
+__device__ __forceinline__ void pad_list(uint64_t* list, uint32_t n) {
+    const uint32_t lane = threadIdx.x & 63u;
+    if (lane < 8) list[n + lane] = 0;
+}
+// The number of entries in a workgroup's padded lists that are larger than key.
+__device__ __forceinline__ uint32_t larger(const uint64_t (*lists)[kWaveList], const uint32_t (&listed)[kWaves], uint64_t key) {
     uint32_t above = 0;
     for (int w = 0; w < kWaves; ++w) {
-        const uint32_t n = listed[w];
-#pragma unroll 4
-        for (uint32_t j = 0; j < n; ++j) above += lists[w][j] > key;
+        for (uint32_t j = 0; j < listed[w]; j += 8) {
+            uint64_t other[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) other[e] = lists[w][j + e];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) above += other[e] > key;
+        }
     }
     return above;
 }
@@ -299,9 +621,17 @@ __device__ __forceinline__ uint32_t larger(const uint64_t (*lists)[kWaveList], c
 // Candidates are the elements that reach a threshold which k elements are known to reach: in the first tile
 // one that k of its 1024 vectors' maxima reach (few more do, by their counts), then the k-th best of that
 // tile.  Every wave collects its own in a list, so nothing waits inside the loop over the other tiles.
-template <typename T, bool MASKED>
+// JOINED: the workgroup that finishes an item's last slice joins them.
+template <typename T, bool MASKED, bool JOINED>
 __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
-    __shared__ uint64_t lists[kWaves][kWaveList];
+    union Lds {
+        uint64_t lists[kWaves][kWaveList];
+        MergeLds merge;
+    };
+    __shared__ __attribute__((aligned(16))) char lds_bytes[JOINED ? sizeof(Lds) : sizeof(uint64_t) * kWaves * kWaveList];
+    Lds& lds = *reinterpret_cast<Lds*>(lds_bytes);
+    auto& lists = lds.lists;
+    __shared__ uint32_t is_last;
     __shared__ uint64_t block_kth;
     __shared__ __attribute__((aligned(16))) uint32_t bins[kBins];
     __shared__ uint32_t listed[kWaves], wave_top[kWaves];
@@ -311,14 +641,20 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
     constexpr uint32_t kTile = tile_of<T>();
 
     const uint32_t row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6);
     const uint32_t k = a.k;
     SliceInfo* info = a.info + static_cast<size_t>(row) * a.slices + slice;
     if (!finite(a.cum[row]) || (a.finished && a.finished[row])) {
         // nothing is looked up in a row that offers nothing by its logits
-        if (threadIdx.x == 0) *info = SliceInfo{0.0, 0, -INFINITY, 0};
+        if (threadIdx.x == 0) {
+            publish(&info->sum, 0);
+            publish(&info->head, 0);
+            publish(&info->max, __float_as_uint(-INFINITY));
+        }
+        if (JOINED) goto done;
         return;
     }
+    {
     const T* x = static_cast<const T*>(a.logits) + static_cast<int64_t>(row) * a.row_stride;
     const uint8_t* mask = MASKED ? reinterpret_cast<const uint8_t*>(a.allowed + static_cast<int64_t>(row) * a.allowed_stride) : nullptr;
     const uint32_t first = slice * a.tiles_per_slice * kTile;
@@ -358,12 +694,12 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
                 if (top[j] >= thr) atomicAdd(&bins[bin_of(o - ordered(top[j]))], 1u);
             __syncthreads();
             const uint32_t reach = end_of_bin(bin_with(bins, k));
-            if (o > kLowestFinite && o - kLowestFinite > reach) thr = from_ordered(o - reach);
+            if (o > kLowestFinite && o - kLowestFinite > reach) thr = uniform(from_ordered(o - reach));
         }
 
         // sum of exponentials relative to the wave's maximum; 2^(d * log2 e) with log2 e in two parts
         if (__any(most > ref)) {
-            const float new_ref = fmaxf(ref, wave_max(most));
+            const float new_ref = fmaxf(ref, wave_max(most));  // a scalar
             if (ref > -INFINITY) sum *= exp(static_cast<double>(ref) - static_cast<double>(new_ref));
             ref = new_ref;
         }
@@ -386,6 +722,10 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
 #pragma unroll
             for (int j = 0; j < kVecs; ++j) {
                 if (!__any(top[j] >= thr)) continue;
+                if (m > kWaveList - 64 - 64 * V) {
+                    over = true;
+                    break;
+                }
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     float v = f[j * V + e];
@@ -393,14 +733,9 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
                     uint32_t token = tile + mine;
                     asm volatile("" : "+v"(v), "+v"(token));  // the keys of all elements would be made ahead, in a register each
                     const uint64_t key = static_cast<uint64_t>(ordered(v)) << 32 | ~(token + j * 64 * V + e);
-                    const bool in = v >= thr && key >= kth;
-                    const uint64_t who = __ballot(in);
-                    const uint32_t c = __popcll(who);
-                    over |= m + c > kWaveList;
-                    if (m + c <= kWaveList) {
-                        if (in) list[m + lanes_before(who)] = key;
-                        m += c;
-                    }
+                    const uint64_t who = __ballot(v >= thr && key >= kth);
+                    if (v >= thr && key >= kth) list[m + lanes_before(who)] = key;
+                    m += __popcll(who);
                 }
             }
             wave_fence();
@@ -408,32 +743,35 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
                 n = m;
                 break;
             }
-            // more than the list holds: with the k-th best of what it holds as the threshold, this tile's
-            // entries are taken again (n <= 192 and k <= 128 of over 448, so every turn leaves many out)
-            kth = kth_key(list, m, k);
+            // more than the list holds: with the k-th best of what it holds as the threshold, the older entries
+            // are sifted and this tile's taken again (of over 320 all but k <= 128 go for good in every turn)
+            kth = uniform(kth_key(list, m, k));
             thr = from_ordered(static_cast<uint32_t>(kth >> 32));
-            wave_fence();
+            n = uniform(keep_from(list, n, kth));
         }
         if (n > k + 64) {
-            kth = max(kth, kth_key(list, n, k));
+            kth = max(kth, uniform(kth_key(list, n, k)));
             thr = from_ordered(static_cast<uint32_t>(kth >> 32));
-            n = keep_from(list, n, kth);
+            n = uniform(keep_from(list, n, kth));
         }
         if (tile == first && tile + kTile < last) {
             if (threadIdx.x == 0) block_kth = 0;
             if (lane == 0) listed[wave] = n;
+            pad_list(list, n);
             __syncthreads();
+            const uint32_t has[kWaves] = {uniform(listed[0]), uniform(listed[1]), uniform(listed[2]), uniform(listed[3])};
             for (uint32_t i = lane; i < n; i += 64)
-                if (larger(lists, listed, list[i]) == k - 1) block_kth = list[i];
+                if (larger(lists, has, list[i]) == k - 1) block_kth = list[i];
             __syncthreads();
-            if (block_kth > kth) {
-                kth = block_kth;
+            if (uniform(block_kth) > kth) {
+                kth = uniform(block_kth);
                 thr = from_ordered(static_cast<uint32_t>(kth >> 32));
             }
         }
     }
 
     const double total = wave_sum(sum);
+    pad_list(list, n);
     if (lane == 0) {
         listed[wave] = n;
         wave_ref[wave] = ref;
@@ -442,16 +780,16 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
     __syncthreads();
     // the four lists as one, sorted: an entry's place is the number of larger ones
     uint64_t* best = a.best + (static_cast<size_t>(row) * a.slices + slice) * k;
-    uint32_t all = 0;
-    for (int w = 0; w < kWaves; ++w) all += listed[w];
+    const uint32_t has[kWaves] = {uniform(listed[0]), uniform(listed[1]), uniform(listed[2]), uniform(listed[3])};
+    const uint32_t all = has[0] + has[1] + has[2] + has[3];
     for (uint32_t i = lane; i < n; i += 64) {
         const uint64_t key = list[i];
-        const uint32_t above = larger(lists, listed, key);
-        if (above < k) best[above] = key;
-        if (above == 0) info->head = key;
+        const uint32_t above = larger(lists, has, key);
+        if (above < k) publish(&best[above], key);
+        if (above == 0) publish(&info->head, key);
     }
-    for (uint32_t i = all + threadIdx.x; i < k; i += kThreads) best[i] = 0;
-    if (all == 0 && threadIdx.x == 0) info->head = 0;
+    for (uint32_t i = all + threadIdx.x; i < k; i += kThreads) publish(&best[i], 0);
+    if (all == 0 && threadIdx.x == 0) publish(&info->head, 0);
     if (wave == 0) {
         float m = fmaxf(fmaxf(wave_ref[0], wave_ref[1]), fmaxf(wave_ref[2], wave_ref[3]));
         double s = 0.0;
@@ -463,206 +801,24 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
         s += __shfl_xor(s, 1);
         s += __shfl_xor(s, 2);
         if (lane == 0) {
-            info->sum = s;
-            info->max = m;
+            publish(&info->sum, static_cast<uint64_t>(__double_as_longlong(s)));
+            publish(&info->max, __float_as_uint(m));
         }
     }
-}
-
-// ---------------------------------------------------------------------------------------------
-// selection, second kernel: one workgroup takes one batch item
-// ---------------------------------------------------------------------------------------------
-// The rows' maxima and sums are joined from their slices, every slice's entries get their scores in
-// 64 bits, and the k best come out in the order (score down, beam up, logit down, token up).
-// Within a beam that is the slices' own order.
-constexpr uint32_t kMergeThreads = 1024;
-constexpr uint32_t kMergeStage = 1024;
-
-struct Entry {
-    uint64_t score;  // ordered64
-    uint64_t rest;   // beam, ~ordered logit, token: smaller is better
-};
-__device__ __forceinline__ bool better(const Entry& p, const Entry& q) {
-    return p.score > q.score || (p.score == q.score && p.rest < q.rest);
-}
-
-struct RowBase {
-    double top, log_sum, cum;
-};
-
-__device__ __forceinline__ double score_of(const RowBase& r, uint64_t key) {
-    return r.cum + ((static_cast<double>(from_ordered(static_cast<uint32_t>(key >> 32))) - r.top) - r.log_sum);
-}
-
-__device__ __forceinline__ Entry entry_of(const RowBase& r, uint32_t beam, uint64_t key) {
-    const uint32_t o = static_cast<uint32_t>(key >> 32), token = ~static_cast<uint32_t>(key);
-    return Entry{ordered64(score_of(r, key)), static_cast<uint64_t>(beam) << 56 | static_cast<uint64_t>(~o) << 24 | token};
-}
-// The k best of from[0..n_from) and stage[0..n) into to[], sorted: an entry's place is the number of better ones.
-__device__ __forceinline__ uint32_t prune(const Entry* from, uint32_t n_from, const Entry* stage, uint32_t n, Entry* to, uint32_t k) {
-    const uint32_t all = n_from + n;
-    for (uint32_t i = threadIdx.x; i < all; i += kMergeThreads) {
-        const Entry e = i < n_from ? from[i] : stage[i - n_from];
-        uint32_t above = 0;
-        for (uint32_t j = 0; j < n_from; ++j) above += better(from[j], e);
-        for (uint32_t j = 0; j < n; ++j) above += better(stage[j], e);
-        if (above < k) to[above] = e;
+    }
+done:
+    if (!JOINED) return;
+    const uint32_t item = row / a.beams, slices = a.beams * a.slices;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every wave's words have arrived
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const uint32_t before = __hip_atomic_fetch_add(&a.arrived[item], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        is_last = before + 1 == slices;
+        if (before + 1 == slices) a.arrived[item] = 0;  // for the next call on the stream
     }
     __syncthreads();
-    return all < k ? all : k;
-}
-
-// Bins of scores by their distance below the best one, four for every power of two from 2^-44 up.
-__device__ __forceinline__ uint32_t bin_of(double best, double score) {
-    const uint32_t b = __float_as_uint(static_cast<float>(best - score)) >> 21;  // exponent and two bits of the fraction
-    constexpr uint32_t kLow = (127 - 44) * 4;
-    return b <= kLow ? 0 : min(b - kLow, kBins - 1);
-}
-
-__global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(SelectArgs a) {
-    extern __shared__ uint32_t heads[];  // bin of every list's best entry, then the lists that are looked into
-    __shared__ RowBase base[kMaxBeams];
-    __shared__ Entry kept_in_turn[2][kMaxK];
-    __shared__ Entry stage[kMergeStage];
-    __shared__ __attribute__((aligned(16))) uint32_t bins[kBins];
-    __shared__ double wave_best[kMergeThreads / 64];
-    __shared__ uint32_t staged, looked;
-    const uint32_t item = blockIdx.x;
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t lists = a.beams * a.slices;
-    const SliceInfo* info = a.info + static_cast<size_t>(item) * lists;
-    const uint64_t* best = a.best + static_cast<size_t>(item) * lists * a.k;
-    uint32_t* look = heads + lists;
-
-    if (threadIdx.x == 0) staged = looked = 0;
-    if (threadIdx.x < kBins) bins[threadIdx.x] = 0;
-    __syncthreads();
-    // rows: a group of lanes each, a power of two that covers the slices
-    uint32_t group = 1;
-    while (group < a.slices && group < 64) group <<= 1;
-    const uint32_t first = threadIdx.x & (group - 1u);
-    double top = -INFINITY;  // the best score among this thread's lists
-    for (uint32_t beam = threadIdx.x / group; beam < a.beams; beam += kMergeThreads / group) {
-        const uint32_t row = item * a.beams + beam;
-        const float cum = a.cum[row];
-        const bool ended = a.finished && a.finished[row];
-        const SliceInfo* mine = info + beam * a.slices;
-        float m = -INFINITY;
-        for (uint32_t s = first; s < a.slices; s += group) m = fmaxf(m, mine[s].max);
-        for (uint32_t o = group >> 1; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-        double sum = 0.0;
-        for (uint32_t s = first; s < a.slices; s += group) {
-            const float ms = mine[s].max;
-            const double p = mine[s].sum;
-            if (ms > -INFINITY || !(p == 0.0)) sum += p * exp(static_cast<double>(ms) - static_cast<double>(m));
-        }
-        for (uint32_t o = group >> 1; o; o >>= 1) sum += __shfl_xor(sum, o);
-        // a NaN or +inf among the allowed logits has made the sum a NaN
-        const bool live = !ended && finite(cum) && finite(m) && sum > 0.0 && sum < INFINITY;
-        const RowBase r{a.normalize ? static_cast<double>(m) : 0.0, a.normalize ? log(sum) : 0.0, live ? static_cast<double>(cum) : -INFINITY};
-        if (live) top = fmax(top, score_of(r, static_cast<uint64_t>(ordered(m)) << 32));
-        if (first == 0) {
-            base[beam] = r;
-            if (ended && finite(cum)) {
-                stage[atomicAdd(&staged, 1u)] = Entry{ordered64(cum), static_cast<uint64_t>(beam) << 56 | static_cast<uint32_t>(a.end_token)};
-                top = fmax(top, static_cast<double>(cum));
-            }
-        }
-    }
-    for (int o = 32; o; o >>= 1) top = fmax(top, __shfl_xor(top, o));
-    if (lane == 0) wave_best[threadIdx.x >> 6] = top;
-    __syncthreads();
-    for (uint32_t w = 0; w < kMergeThreads / 64; ++w) top = fmax(top, wave_best[w]);
-
-    // which lists: those whose best entry is among the k best of all lists' best ones
-    const uint32_t ended_beams = staged;
-    const bool all_lists = lists * a.k <= 2 * kMergeThreads;
-    uint32_t n_look = lists;
-    if (!all_lists) {
-        for (uint32_t l = threadIdx.x; l < lists; l += kMergeThreads) {
-            const uint32_t beam = l / a.slices;
-            const bool live = base[beam].cum > -INFINITY;
-            const uint64_t head = live ? info[l].head : 0;
-            const uint32_t bin = head ? bin_of(top, score_of(base[beam], head)) : kBins;
-            heads[l] = bin;
-            if (bin < kBins) atomicAdd(&bins[bin], 1u);
-        }
-        if (threadIdx.x < ended_beams) atomicAdd(&bins[bin_of(top, from_ordered64(stage[threadIdx.x].score))], 1u);
-        __syncthreads();
-        const uint32_t upto = bin_with(bins, a.k);
-        __syncthreads();
-        for (uint32_t l = threadIdx.x; l < lists; l += kMergeThreads)
-            if (heads[l] <= upto) look[atomicAdd(&looked, 1u)] = l;
-        if (threadIdx.x < kBins) bins[threadIdx.x] = 0;
-        __syncthreads();
-        n_look = looked;
-    }
-    // which entries: those among the k best by the same count
-    const uint32_t some = n_look * a.k;
-    auto entry_at = [&](uint32_t i, uint32_t& beam) -> uint64_t {
-        const uint32_t which = i / a.k, l = all_lists ? which : look[which];
-        beam = l / a.slices;
-        return base[beam].cum > -INFINITY ? best[static_cast<size_t>(l) * a.k + (i - which * a.k)] : 0;
-    };
-    for (uint32_t i = threadIdx.x; i < some; i += kMergeThreads) {
-        uint32_t beam;
-        const uint64_t key = entry_at(i, beam);
-        if (key) atomicAdd(&bins[bin_of(top, score_of(base[beam], key))], 1u);
-    }
-    if (threadIdx.x < ended_beams) atomicAdd(&bins[bin_of(top, from_ordered64(stage[threadIdx.x].score))], 1u);
-    __syncthreads();
-    const uint32_t upto = bin_with(bins, a.k);
-    for (uint32_t i = threadIdx.x; i < some; i += kMergeThreads) {
-        uint32_t beam;
-        const uint64_t key = entry_at(i, beam);
-        if (!key || bin_of(top, score_of(base[beam], key)) > upto) continue;
-        const uint32_t at = atomicAdd(&staged, 1u);
-        if (at < kMergeStage) stage[at] = entry_of(base[beam], beam, key);
-    }
-    __syncthreads();
-    const Entry* kept = kept_in_turn[0];
-    uint32_t n_kept = 0;
-    if (staged <= kMergeStage) {
-        n_kept = prune(kept, 0, stage, staged, kept_in_turn[0], a.k);
-    } else {
-        // very many ties: the lists a few at a time
-        n_kept = prune(kept, 0, stage, ended_beams, kept_in_turn[0], a.k);
-        uint32_t turn = 1;
-        const uint32_t step = kMergeStage / a.k;
-        for (uint32_t l0 = 0; l0 < n_look; l0 += step) {
-            if (threadIdx.x == 0) staged = 0;
-            __syncthreads();
-            const uint32_t now = min(step, n_look - l0) * a.k;
-            for (uint32_t i = threadIdx.x; i < now; i += kMergeThreads) {
-                uint32_t beam;
-                const uint64_t key = entry_at(l0 * a.k + i, beam);
-                if (!key || bin_of(top, score_of(base[beam], key)) > upto) continue;
-                const Entry e = entry_of(base[beam], beam, key);
-                if (n_kept == a.k && !better(e, kept[a.k - 1])) continue;
-                stage[atomicAdd(&staged, 1u)] = e;
-            }
-            __syncthreads();
-            n_kept = prune(kept, n_kept, stage, staged, kept_in_turn[turn], a.k);
-            kept = kept_in_turn[turn];
-            turn ^= 1;
-        }
-    }
-
-    for (uint32_t i = threadIdx.x; i < a.k; i += kMergeThreads) {
-        const size_t at = static_cast<size_t>(item) * a.k + i;
-        float score = -INFINITY;
-        int32_t parent = -1, token = -1;
-        if (i < n_kept) {
-            score = static_cast<float>(from_ordered64(kept[i].score));  // the one rounding of a score
-            parent = static_cast<int32_t>(kept[i].rest >> 56);
-            token = static_cast<int32_t>(kept[i].rest & 0xffffffu);
-        }
-        a.scores[at] = score;
-        a.parents[at] = parent;
-        a.tokens[at] = token;
-        if (a.out_finished)
-            a.out_finished[at] = parent >= 0 && (token == a.end_token || a.finished[item * a.beams + parent]);
-    }
+    if (!is_last) return;
+    merge_item<kThreads, kHeldJoined>(a, item, lds.merge, nullptr);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -888,6 +1044,11 @@ namespace {
 // CUs several times over, and few enough that their k best stay a small part of what is read.
 constexpr uint64_t kSlicesWanted = 1024;
 
+// Calls of at most this many slices are one launch: the last slice of an item joins its item.  That saves the second
+// launch (1 x 4 x 32000: 12.8 us a call as two, 10.3 as one) but makes every slice wait for its words and a
+// counter, which costs more than it saves once the workgroups share CUs (16 x 8 x 65536: 18 us as two, 23 as one).
+constexpr uint32_t kJoinedSlices = 256;
+
 struct Cut {
     uint32_t tiles_per_slice, slices;
 };
@@ -903,7 +1064,10 @@ uint64_t most_slices(uint64_t rows, uint64_t vocab) {
     const uint64_t all = rows * tiles;
     return all < kSlicesWanted + rows ? all : kSlicesWanted + rows;
 }
-uint64_t scratch_of(uint64_t rows, uint64_t vocab, uint64_t k) { return most_slices(rows, vocab) * (sizeof(SliceInfo) + k * 8); }
+uint64_t arrived_bytes(uint64_t batch) { return (batch * 4 + 255) & ~255ull; }
+uint64_t scratch_of(uint64_t batch, uint64_t beams, uint64_t vocab, uint64_t k) {
+    return arrived_bytes(batch) + most_slices(batch * beams, vocab) * (sizeof(SliceInfo) + k * 8);
+}
 
 const char* limits_error(uint32_t max_batch, uint32_t max_beams, uint32_t max_vocab, uint32_t max_k) {
     if (max_batch < 1 || max_batch > (1u << 20)) return "batch must be 1..2^20";
@@ -919,10 +1083,12 @@ bool overlap(const void* p, uint64_t p_bytes, const void* q, uint64_t q_bytes) {
 }
 
 template <typename T>
-void launch_slices(const SelectArgs& a, uint32_t rows, hipStream_t stream) {
-    const dim3 grid(rows * a.slices);
-    if (a.allowed) hipLaunchKernelGGL((beam_slice_kernel<T, true>), grid, dim3(kThreads), 0, stream, a);
-    else hipLaunchKernelGGL((beam_slice_kernel<T, false>), grid, dim3(kThreads), 0, stream, a);
+void launch_slices(const SelectArgs& a, uint32_t rows, bool joined, hipStream_t stream) {
+    const dim3 grid(rows * a.slices), block(kThreads);
+    if (a.allowed && joined) hipLaunchKernelGGL((beam_slice_kernel<T, true, true>), grid, block, 0, stream, a);
+    else if (a.allowed) hipLaunchKernelGGL((beam_slice_kernel<T, true, false>), grid, block, 0, stream, a);
+    else if (joined) hipLaunchKernelGGL((beam_slice_kernel<T, false, true>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((beam_slice_kernel<T, false, false>), grid, block, 0, stream, a);
 }
 
 }  // namespace
@@ -931,7 +1097,7 @@ extern "C" {
 
 size_t radx_hip_beam_scratch_bytes(uint32_t max_batch, uint32_t max_beams, uint32_t max_vocab, uint32_t max_k) {
     if (limits_error(max_batch, max_beams, max_vocab, max_k)) return 0;
-    return scratch_of(static_cast<uint64_t>(max_batch) * max_beams, max_vocab, max_k);
+    return scratch_of(max_batch, max_beams, max_vocab, max_k);
 }
 
 int radx_hip_beam_create(int device, uint32_t max_batch, uint32_t max_beams, uint32_t max_vocab, uint32_t max_k,
@@ -953,6 +1119,8 @@ int radx_hip_beam_create(int device, uint32_t max_batch, uint32_t max_beams, uin
     h->max_k = max_k;
     const hipError_t e = hipMalloc(reinterpret_cast<void**>(&h->scratch), radx_hip_beam_scratch_bytes(max_batch, max_beams, max_vocab, max_k));
     if (e != hipSuccess) { delete h; return fail(e, "hipMalloc(scratch)"); }
+    const hipError_t z = hipMemset(h->scratch, 0, arrived_bytes(max_batch));
+    if (z != hipSuccess) { (void)hipFree(h->scratch); delete h; return fail(z, "hipMemset(scratch)"); }
     *out = h;
     return 0;
 }
@@ -1015,19 +1183,29 @@ int radx_hip_beam_select(radx_hip_beam* h, const radx_hip_beam_select_args* s, v
     const Cut cut = cut_of(rows, s->vocab, size == 4 ? tile_of<float>() : tile_of<BF16>());
     a.slices = cut.slices;
     a.tiles_per_slice = cut.tiles_per_slice;
-    a.info = reinterpret_cast<SliceInfo*>(h->scratch);
-    a.best = reinterpret_cast<uint64_t*>(h->scratch + most_slices(static_cast<uint64_t>(h->max_batch) * h->max_beams, h->max_vocab) * sizeof(SliceInfo));
+    a.k_inverse = static_cast<uint32_t>((0xffffffffull + a.k) / a.k);
+    a.slices_inverse = static_cast<uint32_t>((0xffffffffull + a.slices) / a.slices);
+    a.arrived = reinterpret_cast<uint32_t*>(h->scratch);
+    char* const slices = h->scratch + arrived_bytes(h->max_batch);
+    a.info = reinterpret_cast<SliceInfo*>(slices);
+    a.best = reinterpret_cast<uint64_t*>(slices + most_slices(static_cast<uint64_t>(h->max_batch) * h->max_beams, h->max_vocab) * sizeof(SliceInfo));
     a.scores = s->scores;
     a.parents = s->parents;
     a.tokens = s->tokens;
     a.out_finished = s->out_finished;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const uint32_t n_rows = static_cast<uint32_t>(rows);
-    if (s->dtype == RADX_HIP_F32) launch_slices<float>(a, n_rows, st);
-    else if (s->dtype == RADX_HIP_BF16) launch_slices<BF16>(a, n_rows, st);
-    else launch_slices<_Float16>(a, n_rows, st);
+    const bool joined = n_rows * a.slices <= kJoinedSlices && a.beams * a.slices * a.k <= kHeldJoined * kThreads;
+    if (s->dtype == RADX_HIP_F32) launch_slices<float>(a, n_rows, joined, st);
+    else if (s->dtype == RADX_HIP_BF16) launch_slices<BF16>(a, n_rows, joined, st);
+    else launch_slices<_Float16>(a, n_rows, joined, st);
     RADX_TRY(hipGetLastError());
-    hipLaunchKernelGGL(beam_merge_kernel, dim3(s->batch), dim3(kMergeThreads), 2 * sizeof(uint32_t) * a.beams * a.slices, st, a);
+    if (joined) return 0;
+    const uint32_t lists = a.beams * a.slices;
+    const dim3 items(s->batch), block(kMergeThreads);
+    if (lists * a.k <= 2 * kMergeThreads) hipLaunchKernelGGL(beam_merge_kernel<2>, items, block, 0, st, a);
+    else if (lists * a.k <= kHeldMost * kMergeThreads) hipLaunchKernelGGL(beam_merge_kernel<kHeldMost>, items, block, 0, st, a);
+    else hipLaunchKernelGGL(beam_merge_kernel<0>, items, block, 2 * sizeof(uint32_t) * lists, st, a);
     RADX_TRY(hipGetLastError());
     return 0;
 }
