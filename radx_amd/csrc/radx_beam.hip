@@ -515,8 +515,8 @@ __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// Entries a wave can hold while it looks through a tile: 320, one vector of every lane more, and padding.
-constexpr uint32_t kWaveList = 320 + 512 + 64;
+constexpr uint32_t kWaveList = 256;  // entries a wave's list holds; eight more are padding
+constexpr uint32_t kQueue = 128;     // vectors a wave's queue holds
 
 // The k-th largest of list[0..n), n >= k; the keys are unique and none is 0.  For lists that grew too long only.
 __device__ __forceinline__ uint64_t kth_key(const uint64_t* list, uint32_t n, uint32_t k) {
@@ -573,26 +573,43 @@ struct TilePart {
     uint4 raw[kVecs];
     uint8_t bits[kVecs];
 
-    __device__ __forceinline__ void load(const T* x, const uint8_t* mask, uint32_t at, uint32_t vocab) {
+    // `end`: behind the tile.  Full tiles are plain loads; in the last one the vectors that reach past the row are
+    // fetched by elements.
+    __device__ __forceinline__ void load(const T* x, const uint8_t* mask, uint32_t at, uint32_t end, uint32_t vocab) {
+        constexpr uint32_t V = Vec<T>::n;
+        const bool full = end <= vocab;
 #pragma unroll
-        for (int j = 0; j < kVecs; ++j, at += 64 * Vec<T>::n) {
-            if (at + Vec<T>::n <= vocab) {
-                const Bytes16 b = *reinterpret_cast<const Bytes16*>(x + at);
+        for (uint32_t j = 0; j < kVecs; ++j) {
+            const uint32_t from = at + j * 64 * V;
+            raw[j] = Vec<T>::tail(x, 0);
+            if (full || from + V <= vocab) {
+                const Bytes16 b = *reinterpret_cast<const Bytes16*>(x + from);
                 raw[j] = uint4{b.w[0], b.w[1], b.w[2], b.w[3]};
-            } else {
-                raw[j] = Vec<T>::tail(x + at, at < vocab ? vocab - at : 0);
             }
-            if (MASKED) bits[j] = at < vocab ? mask[at >> 3] : 0;
+            if (MASKED) {
+                bits[j] = 0;
+                if (full || from < vocab) bits[j] = mask[from >> 3];
+            }
+        }
+        if (full) return;
+#pragma unroll
+        for (uint32_t j = 0; j < kVecs; ++j) {
+            const uint32_t from = at + j * 64 * V;
+            if (from < vocab && from + V > vocab) raw[j] = Vec<T>::tail(x + from, vocab - from);
         }
     }
     __device__ __forceinline__ void unpack(uint32_t at, float* f) const {
+        constexpr uint32_t V = Vec<T>::n;
 #pragma unroll
-        for (int j = 0; j < kVecs; ++j, at += 64 * Vec<T>::n) {
-            Vec<T>::unpack(raw[j], f + j * Vec<T>::n);
+        for (uint32_t j = 0; j < kVecs; ++j) {
+            Vec<T>::unpack(raw[j], f + j * V);
             if (MASKED) {
-                const uint32_t b = static_cast<uint32_t>(bits[j]) >> (at & 7u);
+                const uint32_t b = static_cast<uint32_t>(bits[j]) >> (at & 7u);  // a wave's vectors are 64 V apart: at & 7 is the same in all
 #pragma unroll
-                for (int e = 0; e < Vec<T>::n; ++e) f[j * Vec<T>::n + e] = (b >> e) & 1u ? f[j * Vec<T>::n + e] : -INFINITY;
+                for (uint32_t e = 0; e < V; ++e) {
+                    const uint32_t keep = static_cast<uint32_t>(static_cast<int32_t>(b << (31 - e)) >> 31);
+                    f[j * V + e] = __uint_as_float((__float_as_uint(f[j * V + e]) & keep) | (0xff800000u & ~keep));
+                }
             }
         }
     }
@@ -604,7 +621,7 @@ __device__ __forceinline__ void pad_list(uint64_t* list, uint32_t n) {
     if (lane < 8) list[n + lane] = 0;
 }
 // The number of entries in a workgroup's padded lists that are larger than key.
-__device__ __forceinline__ uint32_t larger(const uint64_t (*lists)[kWaveList], const uint32_t (&listed)[kWaves], uint64_t key) {
+__device__ __forceinline__ uint32_t larger(const uint64_t (*lists)[kWaveList + 8], const uint32_t (&listed)[kWaves], uint64_t key) {
     uint32_t above = 0;
     for (int w = 0; w < kWaves; ++w) {
         for (uint32_t j = 0; j < listed[w]; j += 8) {
@@ -620,17 +637,24 @@ __device__ __forceinline__ uint32_t larger(const uint64_t (*lists)[kWaveList], c
 
 // Candidates are the elements that reach a threshold which k elements are known to reach: in the first tile
 // one that k of its 1024 vectors' maxima reach (few more do, by their counts), then the k-th best of that
-// tile.  Every wave collects its own in a list, so nothing waits inside the loop over the other tiles.
+// tile.  Every wave collects its own in a list, so nothing waits inside the loop over the other tiles.  The few
+// vectors that hold a candidate go through a queue, where a wave tests 64 of their elements at a time: a
+// test and a branch for every element of a tile took 15 of 40 us (64 x 8 x 131072 bfloat16, k = 16).
 // JOINED: the workgroup that finishes an item's last slice joins them.
 template <typename T, bool MASKED, bool JOINED>
 __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
+    struct SliceLds {
+        float queue[kWaves][kQueue * Vec<T>::n];
+        uint64_t lists[kWaves][kWaveList + 8];
+        uint32_t queue_token[kWaves][kQueue];
+    };
     union Lds {
-        uint64_t lists[kWaves][kWaveList];
+        SliceLds slice;
         MergeLds merge;
     };
-    __shared__ __attribute__((aligned(16))) char lds_bytes[JOINED ? sizeof(Lds) : sizeof(uint64_t) * kWaves * kWaveList];
+    __shared__ __attribute__((aligned(16))) char lds_bytes[JOINED ? sizeof(Lds) : sizeof(SliceLds)];
     Lds& lds = *reinterpret_cast<Lds*>(lds_bytes);
-    auto& lists = lds.lists;
+    auto& lists = lds.slice.lists;
     __shared__ uint32_t is_last;
     __shared__ uint64_t block_kth;
     __shared__ __attribute__((aligned(16))) uint32_t bins[kBins];
@@ -662,18 +686,50 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
     const uint32_t mine = wave * (kTile / kWaves) + lane * V;
 
     uint64_t* list = lists[wave];
-    uint32_t n = 0;              // entries in it
-    uint64_t kth = 0;            // an entry has to reach it
-    float thr = -FLT_MAX;        // and so an element this
+    float* queue = lds.slice.queue[wave];
+    uint32_t* queue_token = lds.slice.queue_token[wave];
+    uint32_t n = 0, q = 0;       // entries in the list, vectors in the queue
+    uint64_t reach = static_cast<uint64_t>(kLowestFinite) << 32;  // what an entry has to reach
+    float thr = -FLT_MAX;        // and so an element: the logit of `reach`
     double sum = 0.0;            // this lane's share, relative to ref
-    float ref = -INFINITY;       // the wave's maximum so far
+    float ref = -INFINITY;       // the wave's maximum so far (the workgroup's, in the first tile)
+
+    // the queue's vectors in order of their tokens, 64 elements at a time; all of them, or whole rounds only
+    auto empty_queue = [&](bool all) {
+        constexpr uint32_t kRound = 64 / V;
+        wave_fence();
+        uint32_t done = 0;
+        for (; done < q && (all || q - done >= kRound); done += kRound) {
+            if (n > kWaveList - 64) {
+                reach = uniform(kth_key(list, n, k));
+                thr = from_ordered(static_cast<uint32_t>(reach >> 32));
+                n = uniform(keep_from(list, n, reach));
+            }
+            const bool some = done * V + lane < q * V;
+            const float v = queue[done * V + lane];
+            const uint64_t key = static_cast<uint64_t>(ordered(v)) << 32 | ~(queue_token[done + lane / V] + lane % V);
+            const uint64_t who = __ballot(some && key >= reach);
+            if (some && key >= reach) list[n + lanes_before(who)] = key;
+            n += __popcll(who);
+        }
+        wave_fence();
+        if (done < q) {
+            const float v = queue[done * V + lane];
+            const uint32_t token = queue_token[done + lane / V];
+            wave_fence();
+            queue[lane] = v;
+            if (lane % V == 0) queue_token[lane / V] = token;
+            wave_fence();
+        }
+        q = done < q ? q - done : 0;
+    };
 
     TilePart<T, MASKED> next;
-    next.load(x, mask, first + mine, a.vocab);
+    next.load(x, mask, first + mine, first + kTile, a.vocab);
     for (uint32_t tile = first; tile < last; tile += kTile) {
         float f[kVecs * V];
         next.unpack(tile + mine, f);
-        if (tile + kTile < last) next.load(x, mask, tile + kTile + mine, a.vocab);
+        if (tile + kTile < last) next.load(x, mask, tile + kTile + mine, tile + 2 * kTile, a.vocab);
         float top[kVecs];
         float most = -INFINITY;
 #pragma unroll
@@ -693,66 +749,55 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
             for (int j = 0; j < kVecs; ++j)
                 if (top[j] >= thr) atomicAdd(&bins[bin_of(o - ordered(top[j]))], 1u);
             __syncthreads();
-            const uint32_t reach = end_of_bin(bin_with(bins, k));
-            if (o > kLowestFinite && o - kLowestFinite > reach) thr = uniform(from_ordered(o - reach));
+            ref = uniform(from_ordered(o));
+            const uint32_t within = end_of_bin(bin_with(bins, k));
+            if (o > kLowestFinite && o - kLowestFinite > within) {
+                thr = uniform(from_ordered(o - within));
+                reach = static_cast<uint64_t>(uniform(o - within)) << 32;
+            }
         }
 
-        // sum of exponentials relative to the wave's maximum; 2^(d * log2 e) with log2 e in two parts
+        // sum of exponentials relative to the maximum, as powers of two: the rounded factor is 1.3e-8 off log2 e, which
+        // moves the logarithm of the sum by that times the mean distance from the maximum
         if (__any(most > ref)) {
-            const float new_ref = fmaxf(ref, wave_max(most));  // a scalar
-            if (ref > -INFINITY) sum *= exp(static_cast<double>(ref) - static_cast<double>(new_ref));
+            const float new_ref = wave_max(most);
+            sum *= exp(static_cast<double>(ref) - static_cast<double>(new_ref));
             ref = new_ref;
         }
         const float base = ref > -INFINITY ? ref : 0.0f;
-        constexpr float kLog2eHi = 1.44269502162933349609375f, kLog2eLo = 1.92596298909109e-8f;
+        constexpr float kLog2e = 1.44269502162933349609375f;
 #pragma unroll
         for (int j = 0; j < kVecs * V; j += 8) {
             float e[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float d = f[j + i] - base;
-                e[i] = __builtin_amdgcn_exp2f(fmaf(d, kLog2eHi, d * kLog2eLo));
-            }
+            for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f((f[j + i] - base) * kLog2e);
             sum += static_cast<double>(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])));
         }
 
-        while (__any(most >= thr)) {
-            uint32_t m = n;
-            bool over = false;
+        const bool final_tile = tile + kTile >= last;
+        if (__any(most >= thr)) {
 #pragma unroll
             for (int j = 0; j < kVecs; ++j) {
-                if (!__any(top[j] >= thr)) continue;
-                if (m > kWaveList - 64 - 64 * V) {
-                    over = true;
-                    break;
-                }
+                const bool in = top[j] >= thr;  // thr may rise in between
+                const uint64_t who = __ballot(in);
+                if (!who) continue;
+                const uint32_t c = __popcll(who);
+                if (q + c > kQueue) empty_queue(true);
+                if (in) {
+                    const uint32_t slot = q + lanes_before(who);
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    float v = f[j * V + e];
-                    if (!__any(v >= thr)) continue;
-                    uint32_t token = tile + mine;
-                    asm volatile("" : "+v"(v), "+v"(token));  // the keys of all elements would be made ahead, in a register each
-                    const uint64_t key = static_cast<uint64_t>(ordered(v)) << 32 | ~(token + j * 64 * V + e);
-                    const uint64_t who = __ballot(v >= thr && key >= kth);
-                    if (v >= thr && key >= kth) list[m + lanes_before(who)] = key;
-                    m += __popcll(who);
+                    for (int e = 0; e < V; e += 4)
+                        *reinterpret_cast<float4*>(queue + slot * V + e) = float4{f[j * V + e], f[j * V + e + 1], f[j * V + e + 2], f[j * V + e + 3]};
+                    queue_token[slot] = tile + mine + j * 64 * V;
                 }
+                q += c;
             }
-            wave_fence();
-            if (!over) {
-                n = m;
-                break;
-            }
-            // more than the list holds: with the k-th best of what it holds as the threshold, the older entries
-            // are sifted and this tile's taken again (of over 320 all but k <= 128 go for good in every turn)
-            kth = uniform(kth_key(list, m, k));
-            thr = from_ordered(static_cast<uint32_t>(kth >> 32));
-            n = uniform(keep_from(list, n, kth));
         }
-        if (n > k + 64) {
-            kth = max(kth, uniform(kth_key(list, n, k)));
-            thr = from_ordered(static_cast<uint32_t>(kth >> 32));
-            n = uniform(keep_from(list, n, kth));
+        if (q) empty_queue(tile == first || final_tile);
+        // later tiles' tokens are larger: an element that equals the entry to be reached would come behind it
+        if (static_cast<uint32_t>(reach)) {
+            reach = ((reach >> 32) + 1) << 32;
+            thr = from_ordered(static_cast<uint32_t>(reach >> 32));
         }
         if (tile == first && tile + kTile < last) {
             if (threadIdx.x == 0) block_kth = 0;
@@ -763,12 +808,15 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
             for (uint32_t i = lane; i < n; i += 64)
                 if (larger(lists, has, list[i]) == k - 1) block_kth = list[i];
             __syncthreads();
-            if (uniform(block_kth) > kth) {
-                kth = uniform(block_kth);
-                thr = from_ordered(static_cast<uint32_t>(kth >> 32));
+            const uint64_t beyond = ((uniform(block_kth) >> 32) + 1) << 32;
+            if (block_kth && beyond > reach) {
+                reach = beyond;
+                thr = from_ordered(static_cast<uint32_t>(reach >> 32));
             }
         }
     }
+
+    if (n > 2 * k + 32) n = uniform(keep_from(list, n, uniform(kth_key(list, n, k))));
 
     const double total = wave_sum(sum);
     pad_list(list, n);
@@ -784,9 +832,9 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
     const uint32_t all = has[0] + has[1] + has[2] + has[3];
     for (uint32_t i = lane; i < n; i += 64) {
         const uint64_t key = list[i];
-        const uint32_t above = larger(lists, has, key);
-        if (above < k) publish(&best[above], key);
-        if (above == 0) publish(&info->head, key);
+        const uint32_t rank = larger(lists, has, key);
+        if (rank < k) publish(&best[rank], key);
+        if (rank == 0) publish(&info->head, key);
     }
     for (uint32_t i = all + threadIdx.x; i < k; i += kThreads) publish(&best[i], 0);
     if (all == 0 && threadIdx.x == 0) publish(&info->head, 0);
@@ -796,7 +844,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
         if (lane < kWaves) {
             // a wave without a number above -inf has no maximum to scale by; its sum is 0, or a NaN to be passed on
             s = wave_total[lane];
-            if (wave_ref[lane] > -INFINITY) s *= exp(static_cast<double>(wave_ref[lane]) - static_cast<double>(m));
+            if (wave_ref[lane] > -INFINITY && wave_ref[lane] != m) s *= exp(static_cast<double>(wave_ref[lane]) - static_cast<double>(m));
         }
         s += __shfl_xor(s, 1);
         s += __shfl_xor(s, 2);
