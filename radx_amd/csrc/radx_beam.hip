@@ -100,7 +100,8 @@ __device__ __forceinline__ uint64_t uniform(uint64_t v) {
 // i / d by m = ceil(2^32 / d), for i * d < 2^32
 __device__ __forceinline__ uint32_t divided(uint32_t i, uint32_t d, uint32_t m) { return d == 1 ? i : __umulhi(i, m); }
 
-// Elements of one 16-byte vector as floats; tail(): the first n elements at p, -inf behind them.
+// Elements of one 16-byte vector as floats and back; tail(): the first n elements at p, -inf behind them; one(): the
+// i-th element of an array of vectors.
 template <typename T> struct Vec;
 template <> struct Vec<float> {
     static constexpr int n = 4;
@@ -110,6 +111,10 @@ template <> struct Vec<float> {
         f[2] = __uint_as_float(r.z);
         f[3] = __uint_as_float(r.w);
     }
+    static __device__ __forceinline__ uint4 pack(const float* f) {
+        return uint4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+    }
+    static __device__ __forceinline__ float one(const uint4* vectors, uint32_t i) { return reinterpret_cast<const float*>(vectors)[i]; }
     static __device__ __forceinline__ uint4 tail(const float* p, uint32_t n) {
         const uint32_t none = 0xff800000u;
         return uint4{n > 0 ? __float_as_uint(p[0]) : none, n > 1 ? __float_as_uint(p[1]) : none, n > 2 ? __float_as_uint(p[2]) : none, none};
@@ -134,6 +139,15 @@ template <> struct Vec<BF16> : Half16 {
             f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
         }
     }
+    static __device__ __forceinline__ uint4 pack(const float* f) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(f[2 * i]) >> 16 | (__float_as_uint(f[2 * i + 1]) & 0xffff0000u);
+        return uint4{w[0], w[1], w[2], w[3]};
+    }
+    static __device__ __forceinline__ float one(const uint4* vectors, uint32_t i) {
+        return __uint_as_float(static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(vectors)[i]) << 16);
+    }
     static __device__ __forceinline__ uint4 tail(const BF16* p, uint32_t n) { return tail16(&p->bits, n, 0xff80u); }
 };
 template <> struct Vec<_Float16> : Half16 {
@@ -144,6 +158,15 @@ template <> struct Vec<_Float16> : Half16 {
             f[2 * i] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[i])));
             f[2 * i + 1] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[i] >> 16)));
         }
+    }
+    static __device__ __forceinline__ uint4 pack(const float* f) {  // the values are float16's: nothing is rounded
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(f[2 * i], f[2 * i + 1]));
+        return uint4{w[0], w[1], w[2], w[3]};
+    }
+    static __device__ __forceinline__ float one(const uint4* vectors, uint32_t i) {
+        return static_cast<float>(reinterpret_cast<const _Float16*>(vectors)[i]);
     }
     static __device__ __forceinline__ uint4 tail(const _Float16* p, uint32_t n) { return tail16(reinterpret_cast<const uint16_t*>(p), n, 0xfc00u); }
 };
@@ -195,7 +218,6 @@ __device__ __forceinline__ uint32_t end_of_bin(uint32_t bin) {
 // k best logits.
 struct SliceInfo {
     uint64_t sum;    // of exp(x - max): a double's bits
-    uint64_t head;   // the slice's best entry (0: none)
     uint64_t max;    // a float's bits
 };
 
@@ -217,8 +239,9 @@ struct SelectArgs {
     uint32_t beams, vocab, k;
     uint32_t slices, tiles_per_slice;
     uint32_t k_inverse, slices_inverse;  // ceil(2^32 / d), for divided()
+    uint32_t merge_parts_log2;  // threads that the join gives a list
     SliceInfo* info;            // [row][slice]
-    uint64_t* best;             // [row][slice][k]: ordered logit, then ~token; 0: none
+    uint64_t* best;             // [row][slice][k], best first: ordered logit, then ~token; 0: none
     uint32_t* arrived;          // [batch]: slices of an item that are done; 0 between calls
     float* scores;
     int32_t* parents;
@@ -236,8 +259,7 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 // Within a beam that is the slices' own order.
 constexpr uint32_t kMergeStage = 512;
 constexpr uint32_t kMergeThreads = 1024;  // of the join as a kernel of its own
-constexpr uint32_t kHeldJoined = 2;       // entries a thread holds in the join inside the slices' kernel
-constexpr uint32_t kHeldMost = 16;        // and in the one of its own
+constexpr uint32_t kHeld = 2;             // entries a thread of it fetches ahead, where that is all
 
 struct Entry {
     uint64_t score;  // ordered64
@@ -307,42 +329,43 @@ __device__ __forceinline__ uint32_t bin_of(double best, double score) {
     return b <= kLow ? 0 : min(b - kLow, kBins - 1);
 }
 
-__device__ __forceinline__ float max_of(const SliceInfo& s) { return __uint_as_float(static_cast<uint32_t>(published(&s.max))); }
-
-__device__ __forceinline__ double sum_of(const SliceInfo& s) { return __longlong_as_double(static_cast<int64_t>(published(&s.sum))); }
-
 struct MergeLds {
-    uint32_t bins[kBins];
+    uint32_t bins[2][kBins];
     Entry kept[2][kMaxK + 8];
     Entry stage[kMergeStage + 8];
     RowBase base[kMaxBeams];
     float wave_best[16];
-    uint32_t staged, looked;
+    uint32_t staged;
 };
 
-// HELD: every list's entries are held in registers, at most so many a thread.  0: `heads` has room for two words a
-// list, and the lists whose best entry is not among the k best of these are left out.
-template <uint32_t THREADS, uint32_t HELD>
-__device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, MergeLds& lds, uint32_t* heads) {
-    constexpr bool ALL = HELD > 0;
+// A list has merge_parts threads, and a thread every merge_parts-th entry of it.  HELD: a thread has one list at most,
+// and at most so many entries of it, which it fetches ahead.  0: any number of lists.
+template <uint32_t THREADS, uint32_t HELD, bool SAME_LAUNCH>
+__device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, MergeLds& lds) {
+    constexpr bool kAhead = HELD > 0;
+    auto word = [](const uint64_t* p) { return SAME_LAUNCH ? published(p) : *p; };
+    auto max_of = [&](const SliceInfo& s) { return __uint_as_float(static_cast<uint32_t>(word(&s.max))); };
+    auto sum_of = [&](const SliceInfo& s) { return __longlong_as_double(static_cast<int64_t>(word(&s.sum))); };
     RowBase* const base = lds.base;
     Entry* const stage = lds.stage;
-    uint32_t* const bins = lds.bins;
     uint32_t& staged = lds.staged;
-    uint32_t& looked = lds.looked;
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t lists = a.beams * a.slices;
     const SliceInfo* info = a.info + static_cast<size_t>(item) * lists;
     const uint64_t* best = a.best + static_cast<size_t>(item) * lists * a.k;
-    uint32_t* look = heads + lists;
+    const uint32_t parts = 1u << a.merge_parts_log2, part = threadIdx.x & (parts - 1u);
+    const uint32_t first_list = threadIdx.x >> a.merge_parts_log2, list_step = THREADS >> a.merge_parts_log2;
 
-    uint64_t held[ALL ? HELD : 1];
-    if (ALL) {
+    uint64_t held[kAhead ? HELD : 1];
+    if (kAhead) {
 #pragma unroll
-        for (uint32_t r = 0; r < HELD; ++r) held[r] = threadIdx.x + r * THREADS < lists * a.k ? published(&best[threadIdx.x + r * THREADS]) : 0;
+        for (uint32_t r = 0; r < HELD; ++r) {
+            const uint32_t j = part + (r << a.merge_parts_log2);
+            held[r] = first_list < lists && j < a.k ? word(&best[first_list * a.k + j]) : 0;
+        }
     }
-    if (threadIdx.x == 0) staged = looked = 0;
-    if (threadIdx.x < kBins) bins[threadIdx.x] = 0;
+    if (threadIdx.x == 0) staged = 0;
+    if (threadIdx.x < kBins) lds.bins[0][threadIdx.x] = lds.bins[1][threadIdx.x] = 0;
     __syncthreads();
     // rows: a group of lanes each, a power of two that covers the slices
     uint32_t group = 1;
@@ -386,72 +409,50 @@ __device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, M
     const double top = static_cast<double>(most);
 
     const uint32_t ended_beams = staged;
-    uint32_t n_look = lists;
-    uint32_t limit = kBins - 1;  // the bin up to which k lists have their best entry: no other entry is wanted
-    if (HELD == 0 || HELD > 2) {
-        for (uint32_t l = threadIdx.x; l < lists; l += THREADS) {
-            const uint32_t beam = divided(l, a.slices, a.slices_inverse);
-            const uint64_t head = base[beam].cum > -INFINITY ? published(&info[l].head) : 0;
-            const uint32_t bin = head ? bin_of(top, score_of(base[beam], head)) : kBins;
-            if (!ALL) heads[l] = bin;
-            if (bin < kBins) atomicAdd(&bins[bin], 1u);
-        }
-        if (threadIdx.x < ended_beams) atomicAdd(&bins[bin_of(top, from_ordered64(stage[threadIdx.x].score))], 1u);
-        __syncthreads();
-        limit = bin_with(bins, a.k);
-        __syncthreads();
-        if (!ALL)
-            for (uint32_t l = threadIdx.x; l < lists; l += THREADS)
-                if (heads[l] <= limit) look[atomicAdd(&looked, 1u)] = l;
-        if (threadIdx.x < kBins) bins[threadIdx.x] = 0;
-        __syncthreads();
-        if (!ALL) n_look = looked;
-    }
-    // which entries: those among the k best by the same count
-    const uint32_t some = n_look * a.k;
-    auto beam_at = [&](uint32_t i) {
-        const uint32_t which = divided(i, a.k, a.k_inverse);
-        return divided(ALL ? which : look[which], a.slices, a.slices_inverse);
-    };
-    auto key_at = [&](uint32_t i) {
-        const uint32_t which = divided(i, a.k, a.k_inverse);
-        return best[static_cast<size_t>(ALL ? which : look[which]) * a.k + (i - which * a.k)];
-    };
-    auto offered = [&](uint64_t key, uint32_t beam) { return base[beam].cum > -INFINITY && key != 0; };
-    auto count = [&](uint64_t key, uint32_t i) -> uint32_t {
-        if (!key) return kBins;
-        const uint32_t beam = beam_at(i);
-        if (!offered(key, beam)) return kBins;
-        const uint32_t bin = bin_of(top, score_of(base[beam], key));
-        if (bin <= limit) atomicAdd(&bins[bin], 1u);  // most entries are far away, in few bins: their counts would queue
-        return bin;
-    };
-    uint32_t bin_held[ALL ? HELD : 1];
-    if (ALL) {
+    // which entries: those in the bins up to the k-th best one's.  f(entry, its beam, its bin) is called for a list's
+    // entries in the bins up to `last`; they come best first.
+    auto in_list = [&](uint32_t l, uint32_t last, uint32_t most_of_it, auto&& f) {
+        const uint32_t beam = divided(l, a.slices, a.slices_inverse);
+        const RowBase r = base[beam];
+        if (r.cum == -INFINITY) return;
+        if (kAhead) {
 #pragma unroll
-        for (uint32_t r = 0; r < HELD; ++r)
-            if (r * THREADS < some) bin_held[r] = count(held[r], threadIdx.x + r * THREADS);
-    } else {
-        for (uint32_t i = threadIdx.x; i < some; i += THREADS) count(key_at(i), i);
+            for (uint32_t i = 0; i < HELD; ++i) {
+                const uint32_t bin = held[i] && part + (i << a.merge_parts_log2) < most_of_it ? bin_of(top, score_of(r, held[i])) : kBins;
+                if (bin <= last) f(held[i], beam, bin);
+                if (!__any(bin <= last)) break;
+            }
+        } else {
+            for (uint32_t j = part; j < most_of_it; j += parts) {
+                const uint64_t key = word(&best[static_cast<size_t>(l) * a.k + j]);
+                const uint32_t bin = key ? bin_of(top, score_of(r, key)) : kBins;
+                if (bin > last) break;
+                f(key, beam, bin);
+            }
+        }
+    };
+    auto in_lists = [&](uint32_t last, uint32_t most_of_it, auto&& f) {
+        for (uint32_t l = first_list; l < lists; l += list_step) in_list(l, last, most_of_it, f);
+    };
+    uint32_t* const bins = lds.bins[0];
+    const uint32_t ended_bin = threadIdx.x < ended_beams ? bin_of(top, from_ordered64(stage[threadIdx.x].score)) : kBins;
+    uint32_t limit = kBins - 1;
+    if (lists * a.k > 2 * THREADS) {
+        // first by the lists' best entries alone: most others are far away, in few bins, where their counts would queue
+        uint32_t* const heads = lds.bins[1];
+        in_lists(kBins - 1, 1, [&](uint64_t, uint32_t, uint32_t bin) { atomicAdd(&heads[bin], 1u); });
+        if (ended_bin < kBins) atomicAdd(&heads[ended_bin], 1u);
+        __syncthreads();
+        limit = bin_with(heads, a.k);
     }
-    if (threadIdx.x < ended_beams) atomicAdd(&bins[bin_of(top, from_ordered64(stage[threadIdx.x].score))], 1u);
+    in_lists(limit, a.k, [&](uint64_t, uint32_t, uint32_t bin) { atomicAdd(&bins[bin], 1u); });
+    if (ended_bin < kBins) atomicAdd(&bins[ended_bin], 1u);
     __syncthreads();
     const uint32_t upto = min(bin_with(bins, a.k), limit);
-    auto take = [&](uint64_t key, uint32_t beam) {
+    in_lists(upto, a.k, [&](uint64_t key, uint32_t beam, uint32_t) {
         const uint32_t at = atomicAdd(&staged, 1u);
         if (at < kMergeStage) stage[at] = entry_of(base[beam], beam, key);
-    };
-    if (ALL) {
-#pragma unroll
-        for (uint32_t r = 0; r < HELD; ++r)
-            if (r * THREADS < some && bin_held[r] <= upto) take(held[r], beam_at(threadIdx.x + r * THREADS));
-    } else {
-        for (uint32_t i = threadIdx.x; i < some; i += THREADS) {
-            const uint64_t key = key_at(i);
-            const uint32_t beam = beam_at(i);
-            if (offered(key, beam) && bin_of(top, score_of(base[beam], key)) <= upto) take(key, beam);
-        }
-    }
+    });
     __syncthreads();
     Entry* kept = lds.kept[0];
     uint32_t n_kept = 0;
@@ -462,14 +463,14 @@ __device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, M
         n_kept = prune<THREADS>(lds.kept[1], 0, stage, ended_beams, kept, a.k);
         uint32_t turn = 1;
         const uint32_t step = kMergeStage / a.k;
-        for (uint32_t l0 = 0; l0 < n_look; l0 += step) {
+        for (uint32_t l0 = 0; l0 < lists; l0 += step) {
             if (threadIdx.x == 0) staged = 0;
             __syncthreads();
-            const uint32_t now = min(step, n_look - l0) * a.k;
+            const uint32_t now = min(step, lists - l0) * a.k;
             for (uint32_t i = threadIdx.x; i < now; i += THREADS) {
-                const uint64_t key = key_at(l0 * a.k + i);
-                const uint32_t beam = beam_at(l0 * a.k + i);
-                if (!offered(key, beam) || bin_of(top, score_of(base[beam], key)) > upto) continue;
+                const uint32_t l = l0 + divided(i, a.k, a.k_inverse), beam = divided(l, a.slices, a.slices_inverse);
+                const uint64_t key = word(&best[static_cast<size_t>(l0) * a.k + i]);
+                if (!key || base[beam].cum == -INFINITY || bin_of(top, score_of(base[beam], key)) > upto) continue;
                 const Entry e = entry_of(base[beam], beam, key);
                 if (n_kept == a.k && !better(e, kept[a.k - 1])) continue;
                 stage[atomicAdd(&staged, 1u)] = e;
@@ -500,9 +501,8 @@ __device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, M
 
 template <uint32_t HELD>
 __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(SelectArgs a) {
-    extern __shared__ uint32_t heads[];
     __shared__ __attribute__((aligned(16))) MergeLds lds;
-    merge_item<kMergeThreads, HELD>(a, blockIdx.x, lds, heads);
+    merge_item<kMergeThreads, HELD, false>(a, blockIdx.x, lds);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -516,7 +516,7 @@ __device__ __forceinline__ void wave_fence() {
 }
 
 constexpr uint32_t kWaveList = 256;  // entries a wave's list holds; eight more are padding
-constexpr uint32_t kQueue = 128;     // vectors a wave's queue holds
+constexpr uint32_t kQueue = 272;     // vectors a wave's queue holds: a tile's 256, and what a round left
 
 // The k-th largest of list[0..n), n >= k; the keys are unique and none is 0.  For lists that grew too long only.
 __device__ __forceinline__ uint64_t kth_key(const uint64_t* list, uint32_t n, uint32_t k) {
@@ -644,7 +644,7 @@ __device__ __forceinline__ uint32_t larger(const uint64_t (*lists)[kWaveList + 8
 template <typename T, bool MASKED, bool JOINED>
 __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
     struct SliceLds {
-        float queue[kWaves][kQueue * Vec<T>::n];
+        uint4 queue[kWaves][kQueue];
         uint64_t lists[kWaves][kWaveList + 8];
         uint32_t queue_token[kWaves][kQueue];
     };
@@ -672,7 +672,6 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
         // nothing is looked up in a row that offers nothing by its logits
         if (threadIdx.x == 0) {
             publish(&info->sum, 0);
-            publish(&info->head, 0);
             publish(&info->max, __float_as_uint(-INFINITY));
         }
         if (JOINED) goto done;
@@ -686,7 +685,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
     const uint32_t mine = wave * (kTile / kWaves) + lane * V;
 
     uint64_t* list = lists[wave];
-    float* queue = lds.slice.queue[wave];
+    uint4* queue = lds.slice.queue[wave];
     uint32_t* queue_token = lds.slice.queue_token[wave];
     uint32_t n = 0, q = 0;       // entries in the list, vectors in the queue
     uint64_t reach = static_cast<uint64_t>(kLowestFinite) << 32;  // what an entry has to reach
@@ -706,21 +705,21 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
                 n = uniform(keep_from(list, n, reach));
             }
             const bool some = done * V + lane < q * V;
-            const float v = queue[done * V + lane];
+            const float v = Vec<T>::one(queue, done * V + lane);
             const uint64_t key = static_cast<uint64_t>(ordered(v)) << 32 | ~(queue_token[done + lane / V] + lane % V);
             const uint64_t who = __ballot(some && key >= reach);
             if (some && key >= reach) list[n + lanes_before(who)] = key;
             n += __popcll(who);
         }
         wave_fence();
-        if (done < q) {
-            const float v = queue[done * V + lane];
-            const uint32_t token = queue_token[done + lane / V];
+        if (done < q && lane < kRound) {
+            const uint4 v = queue[done + lane];
+            const uint32_t token = queue_token[done + lane];
             wave_fence();
             queue[lane] = v;
-            if (lane % V == 0) queue_token[lane / V] = token;
-            wave_fence();
+            queue_token[lane] = token;
         }
+        wave_fence();
         q = done < q ? q - done : 0;
     };
 
@@ -778,19 +777,15 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
         if (__any(most >= thr)) {
 #pragma unroll
             for (int j = 0; j < kVecs; ++j) {
-                const bool in = top[j] >= thr;  // thr may rise in between
+                const bool in = top[j] >= thr;
                 const uint64_t who = __ballot(in);
                 if (!who) continue;
-                const uint32_t c = __popcll(who);
-                if (q + c > kQueue) empty_queue(true);
                 if (in) {
                     const uint32_t slot = q + lanes_before(who);
-#pragma unroll
-                    for (int e = 0; e < V; e += 4)
-                        *reinterpret_cast<float4*>(queue + slot * V + e) = float4{f[j * V + e], f[j * V + e + 1], f[j * V + e + 2], f[j * V + e + 3]};
+                    queue[slot] = Vec<T>::pack(f + j * V);
                     queue_token[slot] = tile + mine + j * 64 * V;
                 }
-                q += c;
+                q += __popcll(who);
             }
         }
         if (q) empty_queue(tile == first || final_tile);
@@ -834,10 +829,8 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
         const uint64_t key = list[i];
         const uint32_t rank = larger(lists, has, key);
         if (rank < k) publish(&best[rank], key);
-        if (rank == 0) publish(&info->head, key);
     }
     for (uint32_t i = all + threadIdx.x; i < k; i += kThreads) publish(&best[i], 0);
-    if (all == 0 && threadIdx.x == 0) publish(&info->head, 0);
     if (wave == 0) {
         float m = fmaxf(fmaxf(wave_ref[0], wave_ref[1]), fmaxf(wave_ref[2], wave_ref[3]));
         double s = 0.0;
@@ -866,7 +859,7 @@ done:
     }
     __syncthreads();
     if (!is_last) return;
-    merge_item<kThreads, kHeldJoined>(a, item, lds.merge, nullptr);
+    merge_item<kThreads, kHeld, true>(a, item, lds.merge);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1243,17 +1236,25 @@ int radx_hip_beam_select(radx_hip_beam* h, const radx_hip_beam_select_args* s, v
     a.out_finished = s->out_finished;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const uint32_t n_rows = static_cast<uint32_t>(rows);
-    const bool joined = n_rows * a.slices <= kJoinedSlices && a.beams * a.slices * a.k <= kHeldJoined * kThreads;
+    // the join's threads go to the lists evenly, and no list gets more than it has entries
+    const uint32_t lists = a.beams * a.slices;
+    auto parts_log2 = [&](uint32_t threads) {
+        uint32_t log2 = 0;
+        while ((lists << (log2 + 1)) <= threads && (1u << log2) < a.k && log2 < 6) ++log2;
+        return log2;
+    };
+    auto held = [&](uint32_t log2) { return (a.k + (1u << log2) - 1) >> log2; };
+    a.merge_parts_log2 = parts_log2(kThreads);
+    const bool joined = n_rows * a.slices <= kJoinedSlices && lists <= kThreads && held(a.merge_parts_log2) <= kHeld;
+    if (!joined) a.merge_parts_log2 = parts_log2(kMergeThreads);
     if (s->dtype == RADX_HIP_F32) launch_slices<float>(a, n_rows, joined, st);
     else if (s->dtype == RADX_HIP_BF16) launch_slices<BF16>(a, n_rows, joined, st);
     else launch_slices<_Float16>(a, n_rows, joined, st);
     RADX_TRY(hipGetLastError());
     if (joined) return 0;
-    const uint32_t lists = a.beams * a.slices;
     const dim3 items(s->batch), block(kMergeThreads);
-    if (lists * a.k <= 2 * kMergeThreads) hipLaunchKernelGGL(beam_merge_kernel<2>, items, block, 0, st, a);
-    else if (lists * a.k <= kHeldMost * kMergeThreads) hipLaunchKernelGGL(beam_merge_kernel<kHeldMost>, items, block, 0, st, a);
-    else hipLaunchKernelGGL(beam_merge_kernel<0>, items, block, 2 * sizeof(uint32_t) * lists, st, a);
+    if (lists <= kMergeThreads && held(a.merge_parts_log2) <= kHeld) hipLaunchKernelGGL(beam_merge_kernel<kHeld>, items, block, 0, st, a);
+    else hipLaunchKernelGGL(beam_merge_kernel<0>, items, block, 0, st, a);
     RADX_TRY(hipGetLastError());
     return 0;
 }
