@@ -658,7 +658,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
     __shared__ uint32_t is_last;
     __shared__ uint64_t block_kth;
     __shared__ __attribute__((aligned(16))) uint32_t bins[kBins];
-    __shared__ uint32_t listed[kWaves], wave_top[kWaves];
+    __shared__ uint32_t listed[kWaves], wave_top[kWaves], some_count;
     __shared__ float wave_ref[kWaves];
     __shared__ double wave_total[kWaves];
     constexpr int V = Vec<T>::n;
@@ -815,6 +815,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
 
     const double total = wave_sum(sum);
     pad_list(list, n);
+    bins[threadIdx.x] = 0;
     if (lane == 0) {
         listed[wave] = n;
         wave_ref[wave] = ref;
@@ -825,14 +826,39 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
     uint64_t* best = a.best + (static_cast<size_t>(row) * a.slices + slice) * k;
     const uint32_t has[kWaves] = {uniform(listed[0]), uniform(listed[1]), uniform(listed[2]), uniform(listed[3])};
     const uint32_t all = has[0] + has[1] + has[2] + has[3];
-    for (uint32_t i = lane; i < n; i += 64) {
-        const uint64_t key = list[i];
-        const uint32_t rank = larger(lists, has, key);
-        if (rank < k) publish(&best[rank], key);
+    const float m = fmaxf(fmaxf(wave_ref[0], wave_ref[1]), fmaxf(wave_ref[2], wave_ref[3]));
+    if (all <= 2 * k) {
+        for (uint32_t i = lane; i < n; i += 64) {
+            const uint32_t rank = larger(lists, has, list[i]);
+            if (rank < k) publish(&best[rank], list[i]);
+        }
+    } else {
+        // many more than k: first those that are near enough to the largest, by their counts
+        uint64_t* const some = reinterpret_cast<uint64_t*>(lds.slice.queue);
+        const uint32_t o = ordered(m);
+        for (uint32_t i = lane; i < n; i += 64) atomicAdd(&bins[bin_of(o - static_cast<uint32_t>(list[i] >> 32))], 1u);
+        if (threadIdx.x == 0) some_count = 0;
+        __syncthreads();
+        const uint32_t upto = bin_with(bins, k);
+        for (uint32_t i = lane; i < n; i += 64)
+            if (bin_of(o - static_cast<uint32_t>(list[i] >> 32)) <= upto) some[atomicAdd(&some_count, 1u)] = list[i];
+        __syncthreads();
+        const uint32_t count = uniform(some_count);
+        for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+            const uint64_t key = some[i];
+            uint32_t rank = 0;
+            for (uint32_t j = 0; j < count; j += 8) {
+                uint64_t other[8];
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) other[e] = some[j + e];
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) rank += j + e < count && other[e] > key;
+            }
+            if (rank < k) publish(&best[rank], key);
+        }
     }
     for (uint32_t i = all + threadIdx.x; i < k; i += kThreads) publish(&best[i], 0);
     if (wave == 0) {
-        float m = fmaxf(fmaxf(wave_ref[0], wave_ref[1]), fmaxf(wave_ref[2], wave_ref[3]));
         double s = 0.0;
         if (lane < kWaves) {
             // a wave without a number above -inf has no maximum to scale by; its sum is 0, or a NaN to be passed on
