@@ -234,6 +234,7 @@ def beam_reorder(states, parents, into=None, lengths=None, length_dim=None, row_
     if batch == 0 or k == 0:
         return
     table, beams, address = [], None, capi.ADDRESSES.pack
+    like = packed = None
     for i, s in enumerate(states):
         if s.get_device() != dev:
             _on(s, "a state", dev)
@@ -243,15 +244,16 @@ def beam_reorder(states, parents, into=None, lengths=None, length_dim=None, row_
             d = into[i]
             _on(d, "into", dev)
             row = row_dim + len(has) if row_dim < 0 else row_dim
-            want = tuple(batch * k if n == row else size for n, size in enumerate(has))
-            if d.dtype != s.dtype or d.shape != want:
+            if d.dtype != s.dtype or d.shape != tuple(batch * k if n == row else size for n, size in enumerate(has)):
                 raise ValueError("into must have the states' dtypes and shapes, with batch * k rows")
             d_strides = d.stride()
-        rows, packed = _layout(has, strides, d_strides, s.element_size(), row_dim, length_dim, batch)
-        if rows != beams:
-            if beams is not None:
-                raise ValueError("the states have different numbers of rows")
-            beams = rows
+        if like != (has, strides, d_strides, s.dtype):  # states are often alike
+            like = (has, strides, d_strides, s.dtype)
+            rows, packed = _layout(has, strides, d_strides, s.element_size(), row_dim, length_dim, batch)
+            if rows != beams:
+                if beams is not None:
+                    raise ValueError("the states have different numbers of rows")
+                beams = rows
         if packed is not None:
             table.append(address(s.data_ptr(), d.data_ptr()))
             table.append(packed)

@@ -922,9 +922,12 @@ __device__ __forceinline__ uint4 load_bytes(const char* p, uint32_t n) {
     if (n & 1) v.w |= static_cast<uint32_t>(*reinterpret_cast<const uint8_t*>(p)) << 16;
     return v;
 }
+// Stores of whole vectors are nontemporal: the rows are larger than the L2s that would hold them to the kernel's end
+// (934 MB: 181 -> 169 us, 2.8 GB: 546 -> 525, 252 MB: 43 -> 39.5).
 __device__ __forceinline__ void store_bytes(char* p, uint4 v, uint32_t n) {
     if (n >= 16) {
-        *reinterpret_cast<Bytes16*>(p) = Bytes16{{v.x, v.y, v.z, v.w}};
+        typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(1)));
+        __builtin_nontemporal_store(Words{v.x, v.y, v.z, v.w}, reinterpret_cast<Words*>(p));
         return;
     }
     if (n & 8) { *reinterpret_cast<Bytes8*>(p) = Bytes8{{v.x, v.y}}; p += 8; }
