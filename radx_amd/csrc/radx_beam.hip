@@ -995,6 +995,7 @@ struct BacktraceArgs {
     int32_t* out;          // [batch][k][out_stride]
     int64_t out_stride;
     uint32_t total, batch, k;
+    uint32_t k_inverse, quads_inverse;  // for divided()
     uint32_t segments, segment;  // workgroups an item gets, and the steps that each writes
 };
 
@@ -1004,11 +1005,13 @@ struct BacktraceArgs {
 // dependent look-ups becomes one of 2 n / groups + log2(groups), all of them in LDS.  A segment's workgroup
 // walks through everything behind it first, which needs no traffic between workgroups.
 constexpr uint32_t kTraceThreads = 1024;
-constexpr uint32_t kWindow = 32768;  // places in LDS at once
+constexpr uint32_t kWindow = 32768;  // places in LDS at once, of steps that are only walked through
+constexpr uint32_t kOwn = 8192;      // and of steps that are written, whose tokens follow the parents in the same LDS
+constexpr uint32_t kOwnEach = kOwn / kTraceThreads;
 
 __global__ __launch_bounds__(kTraceThreads) void beam_backtrace_kernel(BacktraceArgs a) {
     __shared__ __attribute__((aligned(16))) uint8_t parent_of[kWindow];
-    __shared__ __attribute__((aligned(16))) uint8_t way[kWindow];
+    __shared__ __attribute__((aligned(16))) uint8_t way[kOwn];
     __shared__ uint8_t maps[2][kTraceThreads];
     __shared__ uint8_t entry[2][kMaxK];
     // an XCD's workgroups (every eighth) take neighbouring items with all their segments: a line of a step's
@@ -1016,29 +1019,54 @@ __global__ __launch_bounds__(kTraceThreads) void beam_backtrace_kernel(Backtrace
     const uint32_t xcd = blockIdx.x & 7u, share = gridDim.x >> 3, more = gridDim.x & 7u;
     const uint32_t place = xcd * share + min(xcd, more) + (blockIdx.x >> 3);
     const uint32_t item = place / a.segments, k = a.k;
-    uint32_t wide = 1;
-    while (wide < k) wide <<= 1;
-    const uint32_t groups = kTraceThreads / wide, group = threadIdx.x / wide, j = threadIdx.x & (wide - 1u);
+    const uint32_t wide_log2 = k > 1 ? 32 - __clz(k - 1) : 0, wide = 1u << wide_log2;
+    const uint32_t groups = kTraceThreads >> wide_log2, group = threadIdx.x >> wide_log2, j = threadIdx.x & (wide - 1u);
     uint32_t ends = a.total;
     if (a.steps) ends = min(a.total, static_cast<uint32_t>(max(0, a.steps[item])));
     const uint32_t s0 = (place - item * a.segments) * a.segment, s1 = min(ends, s0 + a.segment);
     if (s0 >= ends) return;
-    const uint32_t window = kWindow / k;
     const size_t step_places = static_cast<size_t>(a.batch) * k;
     uint32_t turn = 0;
     if (threadIdx.x < k) entry[0][threadIdx.x] = static_cast<uint8_t>(threadIdx.x);
     for (uint32_t w1 = ends; w1 > s0;) {
         const bool own = w1 <= s1;
         const uint32_t border = own ? s0 : s1;
+        const uint32_t window = (own ? kOwn : kWindow) / k;
         const uint32_t w0 = w1 - border > window ? w1 - window : border, n = w1 - w0;
-        const int32_t* from = a.parents + w0 * step_places + static_cast<size_t>(item) * k;
+        const size_t origin = w0 * step_places + static_cast<size_t>(item) * k;
+        const int32_t* from = a.parents + origin;
         __syncthreads();
+        // the tokens are on their way while the parents are walked
+        uint32_t token[kOwnEach];
+        if (own) {
+            const int32_t* tokens = a.tokens + origin;
+            if ((k & 3u) == 0) {
+                const uint32_t quads = k >> 2;
+#pragma unroll
+                for (uint32_t r = 0; r < kOwnEach / 4; ++r) {
+                    const uint32_t i = threadIdx.x + r * kTraceThreads;
+                    if (i >= n * quads) continue;
+                    const uint32_t t = divided(i, quads, a.quads_inverse), p = (i - t * quads) * 4;
+                    const Bytes16 v = *reinterpret_cast<const Bytes16*>(tokens + t * step_places + p);
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) token[4 * r + e] = v.w[e];
+                }
+            } else {
+#pragma unroll
+                for (uint32_t r = 0; r < kOwnEach; ++r) {
+                    const uint32_t i = threadIdx.x + r * kTraceThreads;
+                    if (i >= n * k) continue;
+                    const uint32_t t = divided(i, k, a.k_inverse);
+                    token[r] = static_cast<uint32_t>(tokens[t * step_places + (i - t * k)]);
+                }
+            }
+        }
         if ((k & 3u) == 0) {
             // four places at a time; a step's row is whole fours
             const uint32_t quads = k >> 2;
 #pragma unroll 4
             for (uint32_t i = threadIdx.x; i < n * quads; i += kTraceThreads) {
-                const uint32_t t = i / quads, p = (i - t * quads) * 4;
+                const uint32_t t = divided(i, quads, a.quads_inverse), p = (i - t * quads) * 4;
                 const Bytes16 v = *reinterpret_cast<const Bytes16*>(from + t * step_places + p);
                 uint32_t packed = 0;
 #pragma unroll
@@ -1048,7 +1076,7 @@ __global__ __launch_bounds__(kTraceThreads) void beam_backtrace_kernel(Backtrace
         } else {
 #pragma unroll 4
             for (uint32_t i = threadIdx.x; i < n * k; i += kTraceThreads) {
-                const uint32_t t = i / k, p = i - t * k;
+                const uint32_t t = divided(i, k, a.k_inverse), p = i - t * k;
                 const uint32_t v = static_cast<uint32_t>(from[t * step_places + p]);
                 parent_of[i] = static_cast<uint8_t>(v < k ? v : p);
             }
@@ -1086,12 +1114,24 @@ __global__ __launch_bounds__(kTraceThreads) void beam_backtrace_kernel(Backtrace
         turn ^= 1;
         __syncthreads();
         if (own) {
-            const int32_t* tokens = a.tokens + w0 * step_places + static_cast<size_t>(item) * k;
+            uint32_t* const tokens = reinterpret_cast<uint32_t*>(parent_of);
+            if ((k & 3u) == 0) {
+#pragma unroll
+                for (uint32_t r = 0; r < kOwnEach / 4; ++r) {
+                    const uint32_t i = threadIdx.x + r * kTraceThreads;
+                    if (i < n * (k >> 2)) reinterpret_cast<uint4*>(tokens)[i] = uint4{token[4 * r], token[4 * r + 1], token[4 * r + 2], token[4 * r + 3]};
+                }
+            } else {
+#pragma unroll
+                for (uint32_t r = 0; r < kOwnEach; ++r)
+                    if (threadIdx.x + r * kTraceThreads < n * k) tokens[threadIdx.x + r * kTraceThreads] = token[r];
+            }
+            __syncthreads();
             int32_t* out = a.out + static_cast<int64_t>(item) * k * a.out_stride + w0;
-            // sequences are written along their length; the k look-ups of a step hit the same lines
+            // sequences are written along their length
             for (uint32_t t = threadIdx.x; t < n; t += kTraceThreads)
 #pragma unroll 4
-                for (uint32_t p = 0; p < k; ++p) out[p * a.out_stride + t] = tokens[t * step_places + way[t * k + p]];
+                for (uint32_t p = 0; p < k; ++p) out[p * a.out_stride + t] = static_cast<int32_t>(tokens[t * k + way[t * k + p]]);
         }
         w1 = w0;
     }
@@ -1138,6 +1178,8 @@ uint64_t arrived_bytes(uint64_t batch) { return (batch * 4 + 255) & ~255ull; }
 uint64_t scratch_of(uint64_t batch, uint64_t beams, uint64_t vocab, uint64_t k) {
     return arrived_bytes(batch) + most_slices(batch * beams, vocab) * (sizeof(SliceInfo) + k * 8);
 }
+
+uint32_t inverse(uint32_t d) { return static_cast<uint32_t>((0xffffffffull + d) / d); }  // ceil(2^32 / d)
 
 const char* limits_error(uint32_t max_batch, uint32_t max_beams, uint32_t max_vocab, uint32_t max_k) {
     if (max_batch < 1 || max_batch > (1u << 20)) return "batch must be 1..2^20";
@@ -1253,8 +1295,8 @@ int radx_hip_beam_select(radx_hip_beam* h, const radx_hip_beam_select_args* s, v
     const Cut cut = cut_of(rows, s->vocab, size == 4 ? tile_of<float>() : tile_of<BF16>());
     a.slices = cut.slices;
     a.tiles_per_slice = cut.tiles_per_slice;
-    a.k_inverse = static_cast<uint32_t>((0xffffffffull + a.k) / a.k);
-    a.slices_inverse = static_cast<uint32_t>((0xffffffffull + a.slices) / a.slices);
+    a.k_inverse = inverse(a.k);
+    a.slices_inverse = inverse(a.slices);
     a.arrived = reinterpret_cast<uint32_t*>(h->scratch);
     char* const slices = h->scratch + arrived_bytes(h->max_batch);
     a.info = reinterpret_cast<SliceInfo*>(slices);
@@ -1389,12 +1431,13 @@ int radx_hip_beam_backtrace(const int32_t* tokens, const int32_t* parents, const
         return bad_arg("out overlaps an input");
     RADX_ON_DEVICE_OF(out);
     // a workgroup a CU where the sequences are long enough to be cut
-    const uint64_t most = (static_cast<uint64_t>(total_steps) * k + 4095) / 4096;
+    const uint64_t most = (static_cast<uint64_t>(total_steps) * k + kOwn / 2 - 1) / (kOwn / 2);
     uint64_t segments = batch >= 256 ? 1 : 256 / batch;
     if (segments > most) segments = most;
     const uint32_t segment = static_cast<uint32_t>((total_steps + segments - 1) / segments);
     const uint32_t cuts = (total_steps + segment - 1) / segment;
-    const BacktraceArgs a{tokens, parents, steps, out, static_cast<int64_t>(out_stride), total_steps, batch, k, cuts, segment};
+    const BacktraceArgs a{tokens, parents, steps, out, static_cast<int64_t>(out_stride), total_steps, batch, k,
+                          inverse(k), inverse(k >= 4 ? k / 4 : 1), cuts, segment};
     hipLaunchKernelGGL(beam_backtrace_kernel, dim3(cuts * batch), dim3(kTraceThreads), 0, static_cast<hipStream_t>(stream), a);
     RADX_TRY(hipGetLastError());
     return 0;
