@@ -171,15 +171,18 @@ template <> struct Vec<_Float16> : Half16 {
     static __device__ __forceinline__ uint4 tail(const _Float16* p, uint32_t n) { return tail16(reinterpret_cast<const uint16_t*>(p), n, 0xfc00u); }
 };
 
-// Counts by distance below the largest, in bins that grow by 2^(1/PER) or so: whatever the scale of the values,
-// the bins up to the k-th one's hold few more than k.
-constexpr uint32_t kBins = 256;
+// Counts by distance below the largest, in bins that grow by a sixteenth of an octave: whatever the scale of the
+// values, the bins up to the k-th one's hold few more than k (with a quarter of an octave 290 for k = 64).
+constexpr uint32_t kBins = 512;
 // The first bin up to which there are k (the last bin if there are fewer), in every lane of a wave.
 __device__ __forceinline__ uint32_t bin_with(const uint32_t* bins, uint32_t k) {
     const uint32_t lane = threadIdx.x & 63u;
-    const uint4 c = reinterpret_cast<const uint4*>(bins)[lane];
-    const uint32_t c1 = c.x + c.y, c2 = c1 + c.z, c3 = c2 + c.w;
-    uint32_t upto = c3;
+    const uint4 lo = reinterpret_cast<const uint4*>(bins)[2 * lane], hi = reinterpret_cast<const uint4*>(bins)[2 * lane + 1];
+    const uint32_t c[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mine += c[i];
+    uint32_t upto = mine;
 #define RADX_DPP_ADD(ctrl, rows) \
     upto += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(upto), ctrl, rows, 0xf, false))
     RADX_DPP_ADD(0x111, 0xf);  // row_shr:1
@@ -191,22 +194,27 @@ __device__ __forceinline__ uint32_t bin_with(const uint32_t* bins, uint32_t k) {
 #undef RADX_DPP_ADD
     const uint64_t enough = __ballot(upto >= k);
     if (!enough) return kBins - 1;
-    const uint32_t before = upto - c3;
-    const uint32_t at = 4 * lane + (before + c.x >= k ? 0 : before + c1 >= k ? 1 : before + c2 >= k ? 2 : 3);
+    uint32_t before = upto - mine, at = 8 * lane;
+#pragma unroll
+    for (int i = 0; i < 7; ++i) {
+        before += c[i];
+        at += before < k;
+    }
     return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(at), __ffsll(static_cast<unsigned long long>(enough)) - 1));
 }
-// Bins of whole-number distances: 0, and eight for every power of two.
+// Bins of whole-number distances: up to 15 one each, then sixteen for every power of two.
 __device__ __forceinline__ uint32_t bin_of(uint32_t distance) {
-    if (distance < 8) return distance;
+    if (distance < 16) return distance;
     const uint32_t top = 31 - __clz(distance);
-    return (top - 2) * 8 + ((distance >> (top - 3)) & 7u);
+    return (top - 3) * 16 + ((distance >> (top - 4)) & 15u);
 }
 // The largest distance that a bin holds.
 __device__ __forceinline__ uint32_t end_of_bin(uint32_t bin) {
-    if (bin < 8) return bin;
-    const uint32_t top = bin / 8 + 2;
-    const uint64_t end = (8ull + (bin & 7u) + 1) << (top - 3);
-    return end > 0xffffffffull ? 0xffffffffu : static_cast<uint32_t>(end) - 1u;
+    if (bin < 16) return bin;
+    const uint32_t top = bin / 16 + 3;
+    if (top > 31) return 0xffffffffu;
+    const uint64_t end = (16ull + (bin & 15u) + 1) << (top - 4);
+    return static_cast<uint32_t>(end - 1);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -288,11 +296,12 @@ __device__ __forceinline__ Entry entry_of(const RowBase& r, uint32_t beam, uint6
     return Entry{ordered64(score_of(r, key)), static_cast<uint64_t>(beam) << 56 | static_cast<uint64_t>(~o) << 24 | token};
 }
 // The k best of from[0..n_from) and stage[0..n) into to[], sorted: an entry's place is the number of better ones.
-// Arrays have room for eight entries behind their last, which are made the worst there are.
+// Arrays have room for kPad entries behind their last, which are made the worst there are.
+constexpr uint32_t kPad = 64;
 template <uint32_t THREADS>
 __device__ __forceinline__ uint32_t prune(Entry* from, uint32_t n_from, Entry* stage, uint32_t n, Entry* to, uint32_t k) {
     const uint32_t all = n_from + n;
-    if (threadIdx.x < 8) {
+    if (threadIdx.x < kPad) {
         from[n_from + threadIdx.x] = Entry{0, 0};
         stage[n + threadIdx.x] = Entry{0, 0};
     }
@@ -303,10 +312,10 @@ __device__ __forceinline__ uint32_t prune(Entry* from, uint32_t n_from, Entry* s
     const uint32_t part = threadIdx.x & (parts - 1u);
     auto count = [&](const Entry* list, uint32_t size, const Entry& e) {
         uint32_t above = 0;
-        for (uint32_t j = part * 8; j < size; j += parts * 8) {
+        for (uint32_t j = part; j < size; j += parts * 8) {
             Entry other[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) other[i] = list[j + i];
+            for (uint32_t i = 0; i < 8; ++i) other[i] = list[j + i * parts];  // an entry's lanes read neighbours
 #pragma unroll
             for (int i = 0; i < 8; ++i) above += better(other[i], e);
         }
@@ -322,17 +331,17 @@ __device__ __forceinline__ uint32_t prune(Entry* from, uint32_t n_from, Entry* s
     return all < k ? all : k;
 }
 
-// Bins of scores by their distance below the best one, four for every power of two from 2^-44 up.
+// Bins of scores by their distance below the best one, sixteen for every power of two from 2^-24 to 2^8.
 __device__ __forceinline__ uint32_t bin_of(double best, double score) {
-    const uint32_t b = __float_as_uint(static_cast<float>(best - score)) >> 21;  // exponent and two bits of the fraction
-    constexpr uint32_t kLow = (127 - 44) * 4;
+    const uint32_t b = __float_as_uint(static_cast<float>(best - score)) >> 19;  // exponent and four bits of the fraction
+    constexpr uint32_t kLow = (127 - 24) * 16;
     return b <= kLow ? 0 : min(b - kLow, kBins - 1);
 }
 
 struct MergeLds {
     uint32_t bins[2][kBins];
-    Entry kept[2][kMaxK + 8];
-    Entry stage[kMergeStage + 8];
+    Entry kept[2][kMaxK + kPad];
+    Entry stage[kMergeStage + kPad];
     RowBase base[kMaxBeams];
     float wave_best[16];
     uint32_t staged;
@@ -365,7 +374,7 @@ __device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, M
         }
     }
     if (threadIdx.x == 0) staged = 0;
-    if (threadIdx.x < kBins) lds.bins[0][threadIdx.x] = lds.bins[1][threadIdx.x] = 0;
+    for (uint32_t i = threadIdx.x; i < kBins; i += THREADS) lds.bins[0][i] = lds.bins[1][i] = 0;
     __syncthreads();
     // rows: a group of lanes each, a power of two that covers the slices
     uint32_t group = 1;
@@ -741,7 +750,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
         if (tile == first) {
             const float high = wave_max(most);
             if (lane == 0) wave_top[wave] = ordered(high);
-            bins[threadIdx.x] = 0;
+            bins[threadIdx.x] = bins[threadIdx.x + kThreads] = 0;
             __syncthreads();
             const uint32_t o = max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3]));
 #pragma unroll
@@ -815,7 +824,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
 
     const double total = wave_sum(sum);
     pad_list(list, n);
-    bins[threadIdx.x] = 0;
+    bins[threadIdx.x] = bins[threadIdx.x + kThreads] = 0;
     if (lane == 0) {
         listed[wave] = n;
         wave_ref[wave] = ref;
