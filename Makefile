@@ -1,5 +1,5 @@
 # Build recipe for the gfx950 radix-sort engine, the CPU oracle and the harness.
-#   make            -> radx_amd/lib/libradx_hip.so, oracle/libradx_oracle.so, harness/sort_test
+#   make            -> radx_amd/lib/libradx_hip.so, oracle/libradx_oracle.so, harness/sort_test, harness/beam_test, ...
 #   make resources  -> per-kernel VGPR/SGPR/LDS/occupancy report
 HIPCC    ?= /opt/rocm/bin/hipcc
 CC       ?= gcc
@@ -16,8 +16,9 @@ CPUSORT  := oracle/libradx_cpusort.so
 HARNESS  := harness/sort_test
 SHARDED  := harness/sharded_test
 REFSEQ   := harness/reference_sequence
+BEAM     := harness/beam_test
 
-all: $(LIB) $(ORACLE) $(CPUSORT) $(HARNESS) $(SHARDED) $(REFSEQ)
+all: $(LIB) $(ORACLE) $(CPUSORT) $(HARNESS) $(SHARDED) $(REFSEQ) $(BEAM)
 
 ENGINE   := radx_amd/csrc/radx_hip.hip radx_amd/csrc/radx_beam.hip
 
@@ -41,6 +42,13 @@ $(HARNESS): harness/sort_test.cpp $(LIB) $(wildcard include/radx/*.hpp) include/
 $(REFSEQ): harness/reference_sequence.cpp $(LIB) $(wildcard include/radx/*.hpp) include/radx_hip.h
 	$(CXX) -O2 -std=c++17 -Wall -Wextra -Iinclude -I/opt/rocm/include -D__HIP_PLATFORM_AMD__ \
 	    -o $@ harness/reference_sequence.cpp \
+	    -Lradx_amd/lib -lradx_hip -L/opt/rocm/lib -lamdhip64 \
+	    -Wl,-rpath,'$$ORIGIN/../radx_amd/lib' -Wl,-rpath,/opt/rocm/lib
+
+# beam search through the C++ layer, checked against the host
+$(BEAM): harness/beam_test.cpp $(LIB) $(wildcard include/radx/*.hpp) include/radx_hip.h
+	$(CXX) -O2 -std=c++17 -Wall -Wextra -Iinclude -I/opt/rocm/include -D__HIP_PLATFORM_AMD__ \
+	    -o $@ harness/beam_test.cpp \
 	    -Lradx_amd/lib -lradx_hip -L/opt/rocm/lib -lamdhip64 \
 	    -Wl,-rpath,'$$ORIGIN/../radx_amd/lib' -Wl,-rpath,/opt/rocm/lib
 
@@ -80,7 +88,7 @@ tools/micro/copy_bench: tools/micro/copy_bench.hip
 	$(HIPCC) -O3 -w --offload-arch=$(ARCH) $(NOPACKED) -o $@ $<
 
 clean:
-	rm -f $(LIB) $(ORACLE) $(CPUSORT) $(HARNESS) $(SHARDED) $(REFSEQ) tools/micro/copy_bench tools/micro/rocprim_sort_bench \
+	rm -f $(LIB) $(ORACLE) $(CPUSORT) $(HARNESS) $(SHARDED) $(REFSEQ) $(BEAM) tools/micro/copy_bench tools/micro/rocprim_sort_bench \
 	    oracle/asan_driver oracle/radx_oracle_asan.o harness/sort_test_asan
 
 .PHONY: all clean resources micro asan

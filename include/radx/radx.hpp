@@ -10,3 +10,4 @@
 #include "radx_device.hpp"
 #include "radx_buffer.hpp"
 #include "radx_internal.hpp"
+#include "radx_beam.hpp"

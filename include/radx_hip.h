@@ -280,7 +280,7 @@ typedef struct radx_hip_beam radx_hip_beam;
 size_t radx_hip_beam_scratch_bytes(uint32_t max_batch, uint32_t max_beams, uint32_t max_vocab, uint32_t max_k);
 
 /*
- * Create the handle of selections of at most max_batch (1..2^20) items x max_beams (1..64) beams x max_vocab
+ * Create the handle of selections of at most max_batch (1..2^20) items x max_beams (1..64) beams (2^22 rows) x max_vocab
  * (1..2^24) tokens, max_k (1..128) places, on HIP device `device`.  It owns the scratch of the call in flight: one
  * selection may be in flight per handle, also between two captured graphs.
  */
@@ -334,7 +334,7 @@ int radx_hip_beam_select(radx_hip_beam* h, const radx_hip_beam_select_args* args
  * is not touched, rows k.. of an item stay.  Otherwise src and dst must not overlap.  The states of a call must
  * not share bytes with each other.
  * A row is outer[0] x outer[1] pieces, src_outer[] / dst_outer[] bytes apart, of units x unit_bytes contiguous
- * bytes each, at any alignment; rows are src_row / dst_row bytes apart.  lengths (device, [batch], or NULL): of the
+ * bytes each (fewer than 64 GiB a row), at any alignment; rows are src_row / dst_row bytes apart and do not overlap.  lengths (device, [batch], or NULL): of the
  * units of item b only the first lengths[b] move; what lies behind them is neither read nor written.
  */
 typedef struct {

@@ -22,7 +22,7 @@ def _torch():
         f32, i32 = torch.float32, torch.int32
         logits = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
         flags = (torch.bool, torch.uint8)
-        empty, empty_like, raw_stream = torch.empty, torch.empty_like, torch._C._cuda_getCurrentRawStream
+        empty_like, raw_stream = torch.empty_like, torch._C._cuda_getCurrentRawStream
     _torch = lambda: names  # noqa: E731
     return names
 
@@ -30,6 +30,12 @@ def _torch():
 def _stream(stream, index):
     """The handle of a stream, by default the device's current one."""
     return getattr(stream, "cuda_stream", stream) if stream is not None else _torch().raw_stream(index)
+
+
+def _made_on(stream, index):
+    """The context in which a call on another stream makes its outputs, so that their memory is that stream's."""
+    import torch
+    return torch.cuda.stream(stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(stream, device=index))
 
 
 def _on(t, name, index):
@@ -130,15 +136,14 @@ class BeamSelector:
             raise ValueError("k must be 1..%d, got %d" % (capi.BEAM_MAX_K, k))
         size = (batch, k)
         if out is None:
-            scores = cum.new_empty(size)  # the cheapest of torch's ways
-            parents = cum.new_empty(size, dtype=T.i32)
-            tokens = T.empty_like(parents)
-            out = (scores, parents, tokens)
-            at = (scores.data_ptr(), parents.data_ptr(), tokens.data_ptr())
+            if stream is None:
+                out = self._outputs(T, cum, finished, size)
+            else:
+                with _made_on(stream, dev):
+                    out = self._outputs(T, cum, finished, size)
+            at = (out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr())
             if finished_at:
-                ended = finished.new_empty(size)
-                out += (ended,)
-                ended_at = ended.data_ptr()
+                ended_at = out[3].data_ptr()
         else:
             out = tuple(out)
             if len(out) != (3 if finished is None else 4):
@@ -153,6 +158,12 @@ class BeamSelector:
         if code:
             capi.check(code)
         return out
+
+    @staticmethod
+    def _outputs(T, cum, finished, size):
+        parents = cum.new_empty(size, dtype=T.i32)  # new_empty: the cheapest of torch's ways
+        out = (cum.new_empty(size), parents, T.empty_like(parents))
+        return out if finished is None else out + (finished.new_empty(size),)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -280,9 +291,11 @@ def beam_backtrace(tokens, parents, steps=None, out=None, stream=None):
     parents_at = _plain(parents, (T.i32,), shape, "parents", dev)
     steps_at = None if steps is None else _plain(steps, (T.i32,), (batch,), "steps", dev)
     if out is None:
-        out = T.empty((batch, k, total), dtype=T.i32, device=tokens.device)
-        if steps is not None:
-            out.fill_(-1)
+        if stream is not None:
+            with _made_on(stream, dev):
+                return beam_backtrace(tokens, parents, steps, tokens.new_empty((batch, k, total)) if steps is None else
+                                      tokens.new_full((batch, k, total), -1), stream)
+        out = tokens.new_empty((batch, k, total)) if steps is None else tokens.new_full((batch, k, total), -1)
     _on(out, "out", dev)
     strides = out.stride()
     if out.dtype != T.i32 or out.shape != (batch, k, total) or (total > 1 and strides[2] != 1) or \

@@ -1193,6 +1193,7 @@ uint32_t inverse(uint32_t d) { return static_cast<uint32_t>((0xffffffffull + d) 
 const char* limits_error(uint32_t max_batch, uint32_t max_beams, uint32_t max_vocab, uint32_t max_k) {
     if (max_batch < 1 || max_batch > (1u << 20)) return "batch must be 1..2^20";
     if (max_beams < 1 || max_beams > kMaxBeams) return "beams must be 1..64";
+    if (static_cast<uint64_t>(max_batch) * max_beams > (1u << 22)) return "batch x beams must be at most 2^22";
     if (max_vocab < 1 || max_vocab > kMaxVocab) return "vocab must be 1..2^24";
     if (max_k < 1 || max_k > kMaxK) return "k must be 1..128";
     return nullptr;
@@ -1201,6 +1202,22 @@ const char* limits_error(uint32_t max_batch, uint32_t max_beams, uint32_t max_vo
 bool overlap(const void* p, uint64_t p_bytes, const void* q, uint64_t q_bytes) {
     const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
     return p && q && a < b + q_bytes && b < a + p_bytes;
+}
+
+// How a state's rows go to workgroups: threads a piece gets (a power of two, 16 bytes a thread), the parts of a
+// longer piece, and workgroups a batch item.
+struct RowCut {
+    uint32_t threads_log2;
+    uint64_t chunks, blocks;
+};
+RowCut row_cut_of(const radx_hip_beam_state& t) {
+    RowCut c{0, 0, 0};
+    const uint64_t vecs = (t.units * t.unit_bytes + 15) / 16;
+    while (c.threads_log2 < 8 && (1ull << c.threads_log2) < vecs) ++c.threads_log2;
+    c.chunks = (vecs + (1ull << c.threads_log2) - 1) >> c.threads_log2;
+    const uint64_t per_block = kThreads >> c.threads_log2;
+    c.blocks = c.chunks * ((static_cast<uint64_t>(t.outer[0]) * t.outer[1] + per_block - 1) / per_block);
+    return c;
 }
 
 template <typename T>
@@ -1354,6 +1371,7 @@ int radx_hip_beam_reorder(const radx_hip_beam_state* states, uint32_t n_states, 
         const uint64_t piece = t.units * t.unit_bytes;
         if (t.units > (1ull << 40) || t.unit_bytes > (1ull << 40) || piece > (1ull << 40)) return bad_arg("a state's rows are too long");
         if (static_cast<uint64_t>(t.outer[0]) * t.outer[1] > (1u << 24)) return bad_arg("a state has more than 2^24 pieces a row");
+        if (row_cut_of(t).blocks >= 1u << 24) return bad_arg("a state's rows are too long for one call");  // a grid has 2^32 threads
         uint64_t reach[2] = {piece, piece};
         for (int o = 0; o < 2; ++o) {
             reach[0] += (t.outer[o] - 1) * t.src_outer[o];
@@ -1410,15 +1428,10 @@ int radx_hip_beam_reorder(const radx_hip_beam_state* states, uint32_t n_states, 
         }
         d.unit_bytes = t.unit_bytes;
         d.units = t.units;
-        const uint64_t vecs = (t.units * t.unit_bytes + 15) / 16;
-        d.threads_log2 = 0;
-        while (d.threads_log2 < 8 && (1ull << d.threads_log2) < vecs) ++d.threads_log2;
-        const uint64_t chunks = (vecs + (1ull << d.threads_log2) - 1) >> d.threads_log2;
-        const uint64_t per_block = kThreads >> d.threads_log2;
-        const uint64_t need = chunks * ((static_cast<uint64_t>(t.outer[0]) * t.outer[1] + per_block - 1) / per_block);
-        if (need > 0x7fffffffull) return bad_arg("a state is too large for one call");
-        d.chunks = static_cast<uint32_t>(chunks);
-        if (need > blocks) blocks = need;
+        const RowCut cut = row_cut_of(t);
+        d.threads_log2 = cut.threads_log2;
+        d.chunks = static_cast<uint32_t>(cut.chunks);
+        if (cut.blocks > blocks) blocks = cut.blocks;
         ++held;
     }
     return 0;

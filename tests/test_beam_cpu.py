@@ -26,7 +26,7 @@ def select_args(**change):
 
 @pytest.mark.parametrize("change,text", [
     (dict(beams=0), "beams"), (dict(beams=65), "beams"), (dict(vocab=0), "vocab"), (dict(vocab=(1 << 24) + 1), "vocab"),
-    (dict(k=0), "k must"), (dict(k=129), "k must"), (dict(batch=(1 << 20) + 1), "batch"), (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"),
+    (dict(batch=1 << 20, beams=8), "batch x beams"), (dict(k=0), "k must"), (dict(k=129), "k must"), (dict(batch=(1 << 20) + 1), "batch"), (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"),
     (dict(logits=None), "NULL"), (dict(cum=None), "NULL"), (dict(scores=None), "NULL"), (dict(parents=None), "NULL"), (dict(tokens=None), "NULL"),
     (dict(row_stride=999), "row_stride"), (dict(row_stride=1 << 41), "stride out of range"),
     (dict(allowed=BASE + (5 << 30), allowed_stride=31), "allowed_stride"),
@@ -93,7 +93,7 @@ def test_struct_formats_are_the_headers(tmp_path):
 @pytest.mark.parametrize("change,text", [
     (dict(src=None), "NULL"), (dict(dst=None), "NULL"), (dict(src_row=8192), "two layouts"), (dict(dst_row=4095, src_row=4095), "rows overlap"),
     (dict(dst=BASE + 4096), "source and destination overlap"), (dict(dst=BASE + 8 * 4096 - 1), "source and destination overlap"),
-    (dict(units=1 << 41), "too long"), (dict(unit_bytes=1 << 30, units=1 << 30), "too long"), (dict(src_row=1 << 41, dst_row=1 << 41), "out of range"),
+    (dict(units=1 << 41), "too long"), (dict(units=1 << 30, src_row=1 << 37, dst_row=1 << 37), "too long for one call"), (dict(unit_bytes=1 << 30, units=1 << 30), "too long"), (dict(src_row=1 << 41, dst_row=1 << 41), "out of range"),
     (dict(outer=(1 << 13, 1 << 12)), "pieces"), (dict(outer=(2, 1), src_outer=(100, 0), dst_outer=(100, 0)), "pieces overlap"),
     (dict(outer=(2, 1), src_outer=(1 << 41, 0), dst_outer=(1 << 41, 0)), "out of range"),
     (dict(outer=(2, 1), src_outer=(8192, 0), dst_outer=(4096, 0)), "two layouts"),
@@ -130,6 +130,16 @@ def test_backtrace_refuses():
     refused(call(tokens=BASE + 1), "aligned")
     refused(call(out=BASE + 316), "out overlaps")
     refused(call(steps=BASE + (2 << 30)), "out overlaps")
+
+
+def test_the_c_plus_plus_layer_compiles():
+    """harness/beam_test.cpp drives include/radx/radx_beam.hpp; tests/test_gpu_beam.py runs it."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    made = subprocess.run(["make", "-C", root, "-W", "harness/beam_test.cpp", "harness/beam_test"], capture_output=True, text=True, timeout=600)
+    assert made.returncode == 0, made.stdout + made.stderr
+    assert "warning" not in made.stderr, made.stderr
 
 
 def test_host_tensors_are_refused():

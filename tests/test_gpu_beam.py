@@ -354,6 +354,95 @@ def test_select_extreme_logits(device):
     sel.close()
 
 
+@pytest.mark.parametrize("kind", ["clustered", "falling", "rising", "few allowed in one place", "sixteen equal rows"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k", [3, 16, 100])
+def test_select_lists_and_queues(device, kind, dtype, k):
+    """Rows of many tiles whose best values come all at once, ever better, or in few threads' hands: the lists' and
+    queues' limits.  Scores are given, so every one is exact."""
+    import torch
+    import radx_amd
+    batch, beams, vocab = 1, 16, 150001
+    rng = np.random.default_rng(k)
+    x = rng.standard_normal((beams, vocab)).astype(np.float32)
+    if kind == "clustered":
+        for at in (0, 8190, 65536, vocab - 700):
+            x[:, at:at + 700] += 6.0
+    elif kind == "falling":
+        x = np.broadcast_to(-np.arange(vocab, dtype=np.float32) / 1000, x.shape) + x * 1e-3
+    elif kind == "rising":
+        x = np.broadcast_to(np.arange(vocab, dtype=np.float32) / 5000, x.shape) + x * 1e-3
+    elif kind == "sixteen equal rows":
+        x[:] = x[0]
+    allowed = None
+    if kind == "few allowed in one place":
+        allowed = np.zeros((beams, vocab), bool)
+        allowed[:, 99000:99000 + 3000] = True
+    logits = torch.from_numpy(np.ascontiguousarray(x)).to(device).to(torch_dtype(dtype))
+    xv = logits.double().cpu().numpy().reshape(batch, beams, vocab)
+    cum = (-np.arange(beams) % 4 * 0.25).astype(np.float32)[None].copy()
+    sel = radx_amd.BeamSelector(batch, beams, vocab, k)
+    words = None if allowed is None else on(words_of(allowed), device)
+    got = run_select(sel, logits, on(cum, device), k, allowed=words, normalize=False)
+    full = None if allowed is None else allowed[None]
+    want = plain_best(plain_scores(xv, cum, allowed=full, normalize=False), xv, k)
+    assert np.array_equal(got[0], want[0].astype(np.float32)) and np.array_equal(got[1], want[1]) and np.array_equal(got[2], want[2])
+    got = run_select(sel, logits, on(cum, device), k, allowed=words)
+    check_best(got, plain_scores(xv, cum, allowed=full), xv, k, vocab)
+    sel.close()
+
+
+def test_select_past_32_bits(device):
+    """Rows that begin more than 4 GiB into the logits."""
+    import torch
+    import radx_amd
+    batch, beams, vocab, k = 9000, 2, 131072, 4
+    logits = torch.zeros(batch * beams, vocab, dtype=torch.bfloat16, device=device)
+    cum = torch.zeros(batch, beams, device=device)
+    at = torch.arange(batch, device=device) * 7 % vocab
+    logits[torch.arange(batch, device=device) * 2 + 1, at] = 30.0
+    sel = radx_amd.BeamSelector(batch, beams, vocab, k)
+    scores, parents, tokens = sel.select(logits, cum, k, normalize=False)
+    assert bool((tokens[:, 0] == at).all()) and bool((parents[:, 0] == 1).all()) and bool((scores[:, 0] == 30.0).all())
+    assert bool((scores[:, 1:] == 0.0).all()) and bool((parents[:, 1:] == 0).all())
+    assert bool((tokens[:, 1:] == torch.arange(k - 1, device=device)).all())
+    sel.close()
+    del logits
+    torch.cuda.empty_cache()
+
+
+def test_select_two_graphs_one_handle(device):
+    """Two captured graphs of one handle, replayed in turn on one stream with eager calls between them."""
+    import torch
+    import radx_amd
+    batch, beams, k = 2, 4, 8
+    sel = radx_amd.BeamSelector(batch, beams, 60000, k)
+    graphs = []
+    for vocab in (9001, 60000):
+        logits, x = make_logits(batch, beams, vocab, "bf16", device, seed=vocab)
+        cum = (-np.random.default_rng(vocab).random((batch, beams))).astype(np.float32)
+        dev_cum = on(cum, device)
+        sel.select(logits, dev_cum, k)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = sel.select(logits, dev_cum, k)
+        graphs.append((g, out, logits, x, cum, dev_cum, vocab))
+    for turn in range(6):
+        g, out, logits, x, cum, dev_cum, vocab = graphs[turn % 2]
+        for o in out:
+            o.zero_()
+        eager = sel.select(logits, dev_cum, k)
+        g.replay()
+        again = sel.select(logits, dev_cum, k)
+        torch.cuda.synchronize()
+        for o, e, f in zip(out, eager, again):
+            assert torch.equal(o, e) and torch.equal(o, f)
+        check_best([o.cpu().numpy() for o in out], plain_scores(x, cum), x, k, vocab)
+    del graphs
+    sel.close()
+
+
 def test_select_is_the_same_every_time(device):
     """No result hangs on the order in which workgroups or atomics come."""
     import radx_amd
@@ -759,3 +848,13 @@ def test_calls_on_streams_of_their_own(device):
             check_best([o.cpu().numpy() for o in out], plain_scores(x, cum), x, 8, x.shape[2])
     for c in cases:
         c[0].close()
+
+
+def test_c_plus_plus_layer(device):
+    """The C++ layer's search over made-up logits equals the host's, token by token (harness/beam_test.cpp)."""
+    import os
+    import subprocess
+    exe = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "harness", "beam_test")
+    for args in ([], ["--batch", "1", "--beams", "1", "--vocab", "7", "--steps", "3", "--width", "1"], ["--batch", "2", "--beams", "17", "--vocab", "3001", "--steps", "5"]):
+        out = subprocess.run([exe] + args, capture_output=True, text=True, timeout=100)
+        assert out.returncode == 0 and "PASS" in out.stdout, out.stdout + out.stderr
