@@ -967,7 +967,7 @@ __device__ __forceinline__ uint4 load_bytes(const char* p, uint32_t n) {
     return v;
 }
 // Stores of whole vectors are nontemporal: the rows are larger than the L2s that would hold them to the kernel's end
-// (934 MB: 181 -> 169 us, 2.8 GB: 546 -> 525, 252 MB: 43 -> 39.5).
+// (934 MB: 181 -> 166 us, 2.8 GB: 547 -> 525, 252 MB: 45 -> 40).
 __device__ __forceinline__ void store_bytes(char* p, uint4 v, uint32_t n) {
     if (n >= 16) {
         typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(1)));
@@ -989,13 +989,15 @@ __global__ __launch_bounds__(kThreads) void beam_reorder_kernel(ReorderArgs a) {
     const uint32_t per_block = kThreads >> s.threads_log2;
     const uint32_t pieces = s.outer[0] * s.outer[1];
     const uint32_t groups = (pieces + per_block - 1) / per_block;
-    uint32_t b = blockIdx.x;
+    // every eighth workgroup goes to the same XCD: each gets a stretch of a row of its own, so that it walks few pages
+    // (934 MB: 168 -> 135 us, 2.8 GB: 525 -> 512), and not the same stretch of every row, which may be the empty one
+    uint32_t stretch = blockIdx.x & 7u;
+    if ((gridDim.x & 7u) == 0) stretch = (stretch + blockIdx.y + blockIdx.z) & 7u;
+    uint32_t b = stretch * (gridDim.x >> 3) + min(stretch, gridDim.x & 7u) + (blockIdx.x >> 3);
     const uint32_t chunk = b % s.chunks;
     b /= s.chunks;
     const uint32_t group = b % groups;
-    const uint32_t item = b / groups;
-    // blockIdx.z counts the batch
-    if (item) return;
+    if (b / groups) return;  // a state of smaller rows than the call's largest
     const uint32_t batch_item = blockIdx.z;
     const uint32_t piece = group * per_block + (threadIdx.x >> s.threads_log2);
     if (piece >= pieces) return;
