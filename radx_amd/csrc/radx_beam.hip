@@ -241,15 +241,10 @@ __device__ __forceinline__ uint32_t reached_by(const uint32_t (&v)[N], uint32_t 
 // are known.  A slice leaves its maximum, its sum of exponentials relative to that maximum, and its
 // k best logits.
 struct SliceInfo {
-    uint64_t sum;    // of exp(x - max): a double's bits
-    uint64_t max;    // a float's bits
+    double sum;  // of exp(x - max)
+    float max;
+    uint32_t unused;
 };
-
-// What slices leave for the join, where the join may be a workgroup of the same launch on another XCD: words
-// that go through to where every XCD sees them, and are fetched from there.  A fence for all of
-// memory would write back and drop the L2 for every workgroup (16 x 8 x 65536: 36 us instead of 15).
-__device__ __forceinline__ void publish(uint64_t* p, uint64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ uint64_t published(const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 struct SelectArgs {
     const void* logits;
@@ -365,12 +360,9 @@ struct MergeLds {
 
 // A list has merge_parts threads, and a thread every merge_parts-th entry of it.  HELD: a thread has one list at most,
 // and at most so many entries of it, which it fetches ahead.  0: any number of lists.
-template <uint32_t THREADS, uint32_t HELD, bool SAME_LAUNCH>
+template <uint32_t THREADS, uint32_t HELD>
 __device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, MergeLds& lds) {
     constexpr bool kAhead = HELD > 0;
-    auto word = [](const uint64_t* p) { return SAME_LAUNCH ? published(p) : *p; };
-    auto max_of = [&](const SliceInfo& s) { return __uint_as_float(static_cast<uint32_t>(word(&s.max))); };
-    auto sum_of = [&](const SliceInfo& s) { return __longlong_as_double(static_cast<int64_t>(word(&s.sum))); };
     RowBase* const base = lds.base;
     Entry* const stage = lds.stage;
     uint32_t& staged = lds.staged;
@@ -386,7 +378,7 @@ __device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, M
 #pragma unroll
         for (uint32_t r = 0; r < HELD; ++r) {
             const uint32_t j = part + (r << a.merge_parts_log2);
-            held[r] = first_list < lists && j < a.k ? word(&best[first_list * a.k + j]) : 0;
+            held[r] = first_list < lists && j < a.k ? best[first_list * a.k + j] : 0;
         }
     }
     if (threadIdx.x == 0) staged = 0;
@@ -404,16 +396,16 @@ __device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, M
         const SliceInfo* mine = info + beam * a.slices;
         // the first slice of every lane is fetched whole before any is looked at; most rows have no more
         const bool some = first < a.slices;
-        const float m0 = some ? max_of(mine[first]) : -INFINITY;
-        const double s0 = some ? sum_of(mine[first]) : 0.0;
+        const float m0 = some ? mine[first].max : -INFINITY;
+        const double s0 = some ? mine[first].sum : 0.0;
         float m = m0;
-        for (uint32_t s = first + group; s < a.slices; s += group) m = fmaxf(m, max_of(mine[s]));
+        for (uint32_t s = first + group; s < a.slices; s += group) m = fmaxf(m, mine[s].max);
         for (uint32_t o = group >> 1; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
         auto scaled = [&](float ms, double p) {
             return ms > -INFINITY || !(p == 0.0) ? p * exp(static_cast<double>(ms) - static_cast<double>(m)) : 0.0;
         };
         double sum = scaled(m0, s0);
-        for (uint32_t s = first + group; s < a.slices; s += group) sum += scaled(max_of(mine[s]), sum_of(mine[s]));
+        for (uint32_t s = first + group; s < a.slices; s += group) sum += scaled(mine[s].max, mine[s].sum);
         for (uint32_t o = group >> 1; o; o >>= 1) sum += __shfl_xor(sum, o);
         // a NaN or +inf among the allowed logits has made the sum a NaN
         const bool live = !ended && finite(cum) && finite(m) && sum > 0.0 && sum < INFINITY;
@@ -449,7 +441,7 @@ __device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, M
             }
         } else {
             for (uint32_t j = part; j < most_of_it; j += parts) {
-                const uint64_t key = word(&best[static_cast<size_t>(l) * a.k + j]);
+                const uint64_t key = best[static_cast<size_t>(l) * a.k + j];
                 const uint32_t bin = key ? bin_of(top, score_of(r, key)) : kBins;
                 if (bin > last) break;
                 f(key, beam, bin);
@@ -494,7 +486,7 @@ __device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, M
             const uint32_t now = min(step, lists - l0) * a.k;
             for (uint32_t i = threadIdx.x; i < now; i += THREADS) {
                 const uint32_t l = l0 + divided(i, a.k, a.k_inverse), beam = divided(l, a.slices, a.slices_inverse);
-                const uint64_t key = word(&best[static_cast<size_t>(l0) * a.k + i]);
+                const uint64_t key = best[static_cast<size_t>(l0) * a.k + i];
                 if (!key || base[beam].cum == -INFINITY || bin_of(top, score_of(base[beam], key)) > upto) continue;
                 const Entry e = entry_of(base[beam], beam, key);
                 if (n_kept == a.k && !better(e, kept[a.k - 1])) continue;
@@ -527,7 +519,7 @@ __device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, M
 template <uint32_t HELD>
 __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(SelectArgs a) {
     __shared__ __attribute__((aligned(16))) MergeLds lds;
-    merge_item<kMergeThreads, HELD, false>(a, blockIdx.x, lds);
+    merge_item<kMergeThreads, HELD>(a, blockIdx.x, lds);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -696,8 +688,8 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
     if (!finite(a.cum[row]) || (a.finished && a.finished[row])) {
         // nothing is looked up in a row that offers nothing by its logits
         if (threadIdx.x == 0) {
-            publish(&info->sum, 0);
-            publish(&info->max, __float_as_uint(-INFINITY));
+            info->sum = 0.0;
+            info->max = -INFINITY;
         }
         if (JOINED) goto done;
         return;
@@ -874,7 +866,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
     if (all <= 2 * k) {
         for (uint32_t i = lane; i < n; i += 64) {
             const uint32_t rank = larger(lists, has, list[i]);
-            if (rank < k) publish(&best[rank], list[i]);
+            if (rank < k) best[rank] = list[i];
         }
     } else {
         // many more than k: first those that are near enough to the largest, by their counts
@@ -898,10 +890,10 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e) rank += j + e < count && other[e] > key;
             }
-            if (rank < k) publish(&best[rank], key);
+            if (rank < k) best[rank] = key;
         }
     }
-    for (uint32_t i = all + threadIdx.x; i < k; i += kThreads) publish(&best[i], 0);
+    for (uint32_t i = all + threadIdx.x; i < k; i += kThreads) best[i] = 0;
     if (wave == 0) {
         double s = 0.0;
         if (lane < kWaves) {
@@ -912,24 +904,27 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
         s += __shfl_xor(s, 1);
         s += __shfl_xor(s, 2);
         if (lane == 0) {
-            publish(&info->sum, static_cast<uint64_t>(__double_as_longlong(s)));
-            publish(&info->max, __float_as_uint(m));
+            info->sum = s;
+            info->max = m;
         }
     }
     }
 done:
     if (!JOINED) return;
     const uint32_t item = row / a.beams, slices = a.beams * a.slices;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every wave's words have arrived
+    // every wave's stores have reached the XCD's L2 (a barrier alone does not wait for them) before one thread releases
+    // that L2 to whichever workgroup comes last, on whatever XCD; a release by each wave costs 0.9 us, this 0.2
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) {
-        const uint32_t before = __hip_atomic_fetch_add(&a.arrived[item], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const uint32_t before = __hip_atomic_fetch_add(&a.arrived[item], 1u, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_AGENT);
         is_last = before + 1 == slices;
         if (before + 1 == slices) a.arrived[item] = 0;  // for the next call on the stream
     }
     __syncthreads();
     if (!is_last) return;
-    merge_item<kThreads, kHeld, true>(a, item, lds.merge);
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    merge_item<kThreads, kHeld>(a, item, lds.merge);
 }
 
 // ---------------------------------------------------------------------------------------------
