@@ -263,7 +263,7 @@ int radx_hip_permutation(void* in, const void* cache, const uint32_t* ptrs, uint
  * of a descending float order, ties by index), the move of the survivors' states to their new places (rows moved
  * by an index, as in radx_hip_permutation), and the sequences out of the recorded choices.  None of it has a
  * counterpart in the reference.  Every call enqueues its kernels on `stream`, allocates nothing and can be
- * captured into a graph.
+ * captured into a graph.  Strides are at most 2^36.
  */
 #define RADX_HIP_F32 0
 #define RADX_HIP_BF16 1

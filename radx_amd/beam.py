@@ -22,7 +22,9 @@ def _torch():
         f32, i32 = torch.float32, torch.int32
         logits = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
         flags = (torch.bool, torch.uint8)
-        empty_like, raw_stream = torch.empty_like, torch._C._cuda_getCurrentRawStream
+        empty_like = torch.empty_like
+        # the handle alone, which a torch.cuda.Stream would cost a microsecond more for
+        raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
     _torch = lambda: names  # noqa: E731
     return names
 
@@ -225,9 +227,9 @@ def beam_reorder(states, parents, into=None, lengths=None, length_dim=None, row_
     pieces); they must not share memory with each other.  into: as many tensors that get the rows instead (b * k + j),
     apart from the states.  lengths: int32 [batch]; of dimension length_dim only the first lengths[b] positions
     move, what lies behind is neither read nor written."""
-    states = (states,) if hasattr(states, "data_ptr") else states
+    states = (states,) if hasattr(states, "data_ptr") else tuple(states)
     if into is not None:
-        into = (into,) if hasattr(into, "data_ptr") else into
+        into = (into,) if hasattr(into, "data_ptr") else tuple(into)
         if len(into) != len(states):
             raise ValueError("into must hold one tensor for each state")
     T = _torch()

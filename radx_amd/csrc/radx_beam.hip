@@ -236,10 +236,15 @@ __device__ __forceinline__ uint32_t reached_by(const uint32_t (&v)[N], uint32_t 
 // ---------------------------------------------------------------------------------------------
 // selection
 // ---------------------------------------------------------------------------------------------
-// One workgroup takes a slice of one row, and one the slices of an item.  score(row, token) = cum[row] + ((x - M) - log sum exp(x - M)): within a row the order of the scores
-// is the order of the logits, so a slice can be searched for its own k best before M and the sum
-// are known.  A slice leaves its maximum, its sum of exponentials relative to that maximum, and its
-// k best logits.
+// score(row, token) = cum[row] + ((x - M) - log sum exp(x - M)) with the row's maximum M: within a row the order of
+// the scores is the order of the logits, so a part of a row can be searched for its k best before M and
+// the sum are known, and the logits are read once.  A workgroup takes a slice of a row and leaves the
+// slice's maximum, its sum of exponentials relative to that maximum and its k best logits; another joins the
+// slices of an item.  What bounds it, large: reading, and the issue of about seven operations an element beside it
+// (64 x 8 x 131072 bfloat16, k = 16: 30 us for 134 MB, 4.5 TB/s; the loads and maxima alone take 22).  Small: the
+// latency of the two phases (1 x 4 x 32000 float32: 10 us).
+// Exponentials are 32-bit, eight of them are added in 32 bits and from there on in 64; scores are 64-bit and rounded
+// once, so that the order of two candidates of different rows hangs on their rows' sums alone (about 1e-8).
 struct SliceInfo {
     double sum;  // of exp(x - max)
     float max;
@@ -276,7 +281,7 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 // The rows' maxima and sums are joined from their slices, every slice's entries get their scores in
 // 64 bits, and the k best come out in the order (score down, beam up, logit down, token up).
 // Within a beam that is the slices' own order.
-constexpr uint32_t kMergeStage = 512;
+constexpr uint32_t kMergeStage = 512;      // entries that are ranked at once; more than k only by ties and the bins' width
 constexpr uint32_t kMergeThreads = 1024;  // of the join as a kernel of its own
 constexpr uint32_t kHeld = 2;             // entries a thread of it fetches ahead, where that is all
 
@@ -1191,13 +1196,14 @@ struct radx_hip_beam {
 
 namespace {
 
-// Slices of all rows of a call that long vocabularies are cut into: enough workgroups to fill 256
-// CUs several times over, and few enough that their k best stay a small part of what is read.
+// Slices that the rows of a call are cut into: the workgroups that 256 CUs hold at once.  With more, every slice's first
+// threshold and last ranking weigh more, and so does the join (64 x 8 x 131072: 43 us at 1024 slices, 95 at 2048,
+// 74 at 768, when the candidate stage was slower).
 constexpr uint64_t kSlicesWanted = 1024;
 
-// Calls of at most this many slices are one launch: the last slice of an item joins its item.  That saves the second
-// launch (1 x 4 x 32000: 12.8 us a call as two, 10.3 as one) but makes every slice wait for its words and a
-// counter, which costs more than it saves once the workgroups share CUs (16 x 8 x 65536: 18 us as two, 23 as one).
+// Calls of at most this many slices, one a CU, are one launch: the last slice of an item joins its item.  That saves the
+// second launch (1 x 4 x 32000: 11.5 us a call as two, 9.9 as one) but makes every slice wait for its stores and
+// a counter, which costs more than it saves once the workgroups share CUs (16 x 8 x 65536: 15 us as two, 22 as one).
 constexpr uint32_t kJoinedSlices = 256;
 
 struct Cut {
@@ -1205,7 +1211,8 @@ struct Cut {
 };
 Cut cut_of(uint64_t rows, uint64_t vocab, uint64_t tile) {
     const uint64_t tiles = (vocab + tile - 1) / tile;
-    const uint64_t per = rows * tiles <= kSlicesWanted ? 1 : (rows * tiles + kSlicesWanted - 1) / kSlicesWanted;
+    uint64_t per = rows * tiles <= kSlicesWanted ? 1 : (rows * tiles + kSlicesWanted - 1) / kSlicesWanted;
+    if (per > tiles) per = tiles;
     return Cut{static_cast<uint32_t>(per), static_cast<uint32_t>((tiles + per - 1) / per)};
 }
 
@@ -1230,6 +1237,8 @@ const char* limits_error(uint32_t max_batch, uint32_t max_beams, uint32_t max_vo
     if (max_k < 1 || max_k > kMaxK) return "k must be 1..128";
     return nullptr;
 }
+
+constexpr uint64_t kMaxStride = 1ull << 36;  // of elements or bytes: extents stay below 2^63
 
 bool overlap(const void* p, uint64_t p_bytes, const void* q, uint64_t q_bytes) {
     const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
@@ -1318,7 +1327,7 @@ int radx_hip_beam_select(radx_hip_beam* h, const radx_hip_beam_select_args* s, v
     if (s->row_stride != 0 && s->row_stride < s->vocab) return bad_arg("row_stride must be 0 or at least vocab");
     const uint64_t words = (static_cast<uint64_t>(s->vocab) + 31) / 32;
     if (s->allowed && s->allowed_stride != 0 && s->allowed_stride < words) return bad_arg("allowed_stride must be 0 or at least ceil(vocab / 32)");
-    if (s->row_stride > (1ull << 40) || s->allowed_stride > (1ull << 40)) return bad_arg("stride out of range");
+    if (s->row_stride > kMaxStride || s->allowed_stride > kMaxStride) return bad_arg("stride out of range");
     if (reinterpret_cast<uintptr_t>(s->logits) % size || reinterpret_cast<uintptr_t>(s->cum) % 4 || reinterpret_cast<uintptr_t>(s->allowed) % 4 ||
         reinterpret_cast<uintptr_t>(s->scores) % 4 || reinterpret_cast<uintptr_t>(s->parents) % 4 || reinterpret_cast<uintptr_t>(s->tokens) % 4)
         return bad_arg("buffer is not aligned to its elements");
@@ -1393,6 +1402,8 @@ int radx_hip_beam_reorder(const radx_hip_beam_state* states, uint32_t n_states, 
     if (src_beams < 1 || dst_beams < 1 || k < 1 || k > RADX_HIP_BEAM_MAX_ROWS) return bad_arg("k must be 1..64, beams at least 1");
     if (k > dst_beams) return bad_arg("k exceeds the rows of a batch item");
     if (batch > 65535) return bad_arg("batch must be < 2^16");
+    if (static_cast<uint64_t>(batch) * src_beams > (1u << 24) || static_cast<uint64_t>(batch) * dst_beams > (1u << 24))
+        return bad_arg("a state has more than 2^24 rows");
     if (batch == 0 || n_states == 0) return 0;
     if (!states || !parents) return bad_arg("NULL argument");
     if (reinterpret_cast<uintptr_t>(parents) % 4 || reinterpret_cast<uintptr_t>(lengths) % 4) return bad_arg("buffer is not aligned to its elements");
@@ -1401,18 +1412,18 @@ int radx_hip_beam_reorder(const radx_hip_beam_state* states, uint32_t n_states, 
         if (t.units == 0 || t.unit_bytes == 0 || t.outer[0] == 0 || t.outer[1] == 0) continue;
         if (!t.src || !t.dst) return bad_arg("a state is NULL");
         const uint64_t piece = t.units * t.unit_bytes;
-        if (t.units > (1ull << 40) || t.unit_bytes > (1ull << 40) || piece > (1ull << 40)) return bad_arg("a state's rows are too long");
+        if (t.units > kMaxStride || t.unit_bytes > kMaxStride || t.units > kMaxStride / t.unit_bytes) return bad_arg("a state's rows are too long");
         if (static_cast<uint64_t>(t.outer[0]) * t.outer[1] > (1u << 24)) return bad_arg("a state has more than 2^24 pieces a row");
         if (row_cut_of(t).blocks >= 1u << 24) return bad_arg("a state's rows are too long for one call");  // a grid has 2^32 threads
         uint64_t reach[2] = {piece, piece};
         for (int o = 0; o < 2; ++o) {
             reach[0] += (t.outer[o] - 1) * t.src_outer[o];
             reach[1] += (t.outer[o] - 1) * t.dst_outer[o];
-            if (t.outer[o] > 1 && (t.src_outer[o] > (1ull << 40) || t.dst_outer[o] > (1ull << 40))) return bad_arg("a state's stride is out of range");
+            if (t.outer[o] > 1 && (t.src_outer[o] > kMaxStride || t.dst_outer[o] > kMaxStride)) return bad_arg("a state's stride is out of range");
             if (t.outer[o] > 1 && t.dst_outer[o] < piece) return bad_arg("a state's pieces overlap");
         }
         if (t.dst_row < piece && static_cast<uint64_t>(batch) * dst_beams > 1) return bad_arg("a state's rows overlap");
-        if (t.src_row > (1ull << 40) || t.dst_row > (1ull << 40)) return bad_arg("a state's stride is out of range");
+        if (t.src_row > kMaxStride || t.dst_row > kMaxStride) return bad_arg("a state's stride is out of range");
         const bool same = t.src == t.dst;
         if (same && (t.src_row != t.dst_row || src_beams != dst_beams || t.src_outer[0] != t.dst_outer[0] || t.src_outer[1] != t.dst_outer[1]))
             return bad_arg("a state in place has two layouts");
@@ -1476,7 +1487,7 @@ int radx_hip_beam_backtrace(const int32_t* tokens, const int32_t* parents, const
     if (total_steps >= (1u << 24)) return bad_arg("total_steps must be < 2^24");
     if (batch == 0 || total_steps == 0) return 0;
     if (!tokens || !parents || !out) return bad_arg("NULL buffer");
-    if (out_stride < total_steps || out_stride > (1ull << 40)) return bad_arg("out_stride must be at least total_steps");
+    if (out_stride < total_steps || out_stride > kMaxStride) return bad_arg("out_stride must be at least total_steps");
     for (const void* p : {static_cast<const void*>(tokens), static_cast<const void*>(parents), static_cast<const void*>(steps), static_cast<const void*>(out)})
         if (reinterpret_cast<uintptr_t>(p) % 4) return bad_arg("buffer is not aligned to its elements");
     const uint64_t places = static_cast<uint64_t>(batch) * k, in_bytes = places * total_steps * 4;

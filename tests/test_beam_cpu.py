@@ -28,7 +28,7 @@ def select_args(**change):
     (dict(beams=0), "beams"), (dict(beams=65), "beams"), (dict(vocab=0), "vocab"), (dict(vocab=(1 << 24) + 1), "vocab"),
     (dict(batch=1 << 20, beams=8), "batch x beams"), (dict(k=0), "k must"), (dict(k=129), "k must"), (dict(batch=(1 << 20) + 1), "batch"), (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"),
     (dict(logits=None), "NULL"), (dict(cum=None), "NULL"), (dict(scores=None), "NULL"), (dict(parents=None), "NULL"), (dict(tokens=None), "NULL"),
-    (dict(row_stride=999), "row_stride"), (dict(row_stride=1 << 41), "stride out of range"),
+    (dict(row_stride=999), "row_stride"), (dict(row_stride=1 << 41), "stride out of range"), (dict(row_stride=(1 << 36) + 1), "stride out of range"),
     (dict(allowed=BASE + (5 << 30), allowed_stride=31), "allowed_stride"),
     (dict(finished=BASE + (5 << 30)), "go together"), (dict(out_finished=BASE + (5 << 30)), "go together"),
     (dict(finished=BASE + (5 << 30), out_finished=BASE + (6 << 30), end_token=-1), "end_token"),
@@ -108,6 +108,7 @@ def test_reorder_refuses_calls():
     refused(reorder([state()], k=5), "exceeds the rows")
     refused(reorder([state()], src=0), "beams")
     refused(reorder([state()], batch=65536), "batch")
+    refused(reorder([state()], batch=1 << 10, src=1 << 15, dst=1 << 15), "2^24 rows")
     refused(reorder([state()], parents=None), "NULL")
     refused(reorder([state()], parents=BASE + 2), "aligned")
     refused(reorder([state(), state()]), "written twice")
@@ -127,6 +128,7 @@ def test_backtrace_refuses():
     refused(call(parents=None), "NULL")
     refused(call(out=None), "NULL")
     refused(call(stride=9), "out_stride")
+    refused(call(stride=(1 << 36) + 1), "out_stride")
     refused(call(tokens=BASE + 1), "aligned")
     refused(call(out=BASE + 316), "out overlaps")
     refused(call(steps=BASE + (2 << 30)), "out overlaps")

@@ -411,6 +411,21 @@ def test_select_past_32_bits(device):
     torch.cuda.empty_cache()
 
 
+def test_select_very_many_rows(device):
+    """More rows than slices are wanted, each of several tiles, all of them one row in memory."""
+    import torch
+    import radx_amd
+    batch, beams, vocab, k = 40000, 64, 20000, 1
+    row = torch.zeros(1, vocab, dtype=torch.bfloat16, device=device)
+    row[0, 19999] = 4.0
+    cum = torch.zeros(batch, beams, device=device)
+    cum[:, 63] = 1.0
+    sel = radx_amd.BeamSelector(batch, beams, vocab, k)
+    scores, parents, tokens = sel.select(row.expand(batch * beams, vocab), cum, k, normalize=False)
+    assert bool((tokens == 19999).all()) and bool((parents == 63).all()) and bool((scores == 5.0).all())
+    sel.close()
+
+
 def test_select_two_graphs_one_handle(device):
     """Two captured graphs of one handle, replayed in turn on one stream with eager calls between them."""
     import torch
