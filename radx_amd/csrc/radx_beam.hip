@@ -538,7 +538,7 @@ __device__ __forceinline__ void wave_fence() {
 }
 
 constexpr uint32_t kWaveList = 256;  // entries a wave's list holds; eight more are padding
-constexpr uint32_t kQueue = 272;     // vectors a wave's queue holds: a tile's 256, and what a round left
+constexpr uint32_t kQueue = 288;     // vectors a wave's queue holds: a tile's 256, and what was too few to look through
 
 // The k-th largest of list[0..n), n >= k; the keys are unique and none is 0.  For lists that grew too long only.
 __device__ __forceinline__ uint64_t kth_key(const uint64_t* list, uint32_t n, uint32_t k) {
@@ -605,8 +605,10 @@ struct TilePart {
             const uint32_t from = at + j * 64 * V;
             raw[j] = Vec<T>::tail(x, 0);
             if (full || from + V <= vocab) {
-                const Bytes16 b = *reinterpret_cast<const Bytes16*>(x + from);
-                raw[j] = uint4{b.w[0], b.w[1], b.w[2], b.w[3]};
+                // read once: nontemporal (64 x 8 x 131072, logits not in any cache: 40 -> 39 us)
+                typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(1)));
+                const Words w = __builtin_nontemporal_load(reinterpret_cast<const Words*>(x + from));
+                raw[j] = uint4{w.x, w.y, w.z, w.w};
             }
             if (MASKED) {
                 bits[j] = 0;
@@ -716,8 +718,8 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
     float ref = -INFINITY;       // the wave's maximum so far (the workgroup's, in the first tile)
 
     // the queue's vectors in order of their tokens, 64 elements at a time; all of them, or whole rounds only
+    constexpr uint32_t kRound = 64 / V;
     auto empty_queue = [&](bool all) {
-        constexpr uint32_t kRound = 64 / V;
         wave_fence();
         uint32_t done = 0;
         for (; done < q && (all || q - done >= kRound); done += kRound) {
@@ -829,7 +831,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
                 q += __popcll(who[j]);
             }
         }
-        if (q) empty_queue(tile == first || final_tile);
+        if (q >= 2 * kRound || (q && (tile == first || final_tile))) empty_queue(tile == first || final_tile);
         // later tiles' tokens are larger: an element that equals the entry to be reached would come behind it
         if (static_cast<uint32_t>(reach)) {
             reach = ((reach >> 32) + 1) << 32;
@@ -1197,8 +1199,8 @@ struct radx_hip_beam {
 namespace {
 
 // Slices that the rows of a call are cut into: the workgroups that 256 CUs hold at once.  With more, every slice's first
-// threshold and last ranking weigh more, and so does the join (64 x 8 x 131072: 43 us at 1024 slices, 95 at 2048,
-// 74 at 768, when the candidate stage was slower).
+// threshold and last ranking weigh more, and so does the join; with fewer, CUs have too little in flight (64 x 8 x
+// 131072, a call: 34 us at 1024 slices, 46 at 768, 39 at 1536, 37 at 2048).
 constexpr uint64_t kSlicesWanted = 1024;
 
 // Calls of at most this many slices, one a CU, are one launch: the last slice of an item joins its item.  That saves the
