@@ -241,7 +241,7 @@ __device__ __forceinline__ uint32_t reached_by(const uint32_t (&v)[N], uint32_t 
 // the sum are known, and the logits are read once.  A workgroup takes a slice of a row and leaves the
 // slice's maximum, its sum of exponentials relative to that maximum and its k best logits; another joins the
 // slices of an item.  What bounds it, large: reading, and the issue of about seven operations an element beside it
-// (64 x 8 x 131072 bfloat16, k = 16: 30 us for 134 MB, 4.5 TB/s; the loads and maxima alone take 22).  Small: the
+// (64 x 8 x 131072 bfloat16, k = 16: 33 us for 134 MB, 4.1 TB/s; the loads and maxima alone take 26).  Small: the
 // latency of the two phases (1 x 4 x 32000 float32: 10 us).
 // Exponentials are 32-bit, eight of them are added in 32 bits and from there on in 64; scores are 64-bit and rounded
 // once, so that the order of two candidates of different rows hangs on their rows' sums alone (about 1e-8).
