@@ -5,7 +5,8 @@ include/radx_hip.h.  A decoding step is
     beam_reorder(states, parents)                               # their states to their places
 
 and after the last one beam_backtrace(tokens, parents) gives the sequences.  torch is used for device
-memory and streams only; the work happens in the library's kernels.
+memory and streams only; the work happens in the library's kernels.  As for the sort, torch is imported before this
+package: it brings a HIP runtime of its own, which the library then shares.
 """
 import ctypes
 import functools

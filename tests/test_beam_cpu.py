@@ -3,6 +3,7 @@ at a device, so addresses that are never read do for buffers."""
 import ctypes
 
 import pytest
+import torch  # noqa: F401  before the library: a process has one HIP runtime, and torch brings its own
 
 import radx_amd
 from radx_amd import capi
