@@ -334,7 +334,8 @@ int radx_hip_beam_select(radx_hip_beam* h, const radx_hip_beam_select_args* args
  * is not touched, rows k.. of an item stay.  Otherwise src and dst must not overlap.  The states of a call must
  * not share bytes with each other.
  * A row is outer[0] x outer[1] pieces, src_outer[] / dst_outer[] bytes apart, of units x unit_bytes contiguous
- * bytes each (fewer than 64 GiB a row), at any alignment; rows are src_row / dst_row bytes apart and do not overlap.  lengths (device, [batch], or NULL): of the
+ * bytes each (fewer than 64 GiB a row), at any alignment; rows are src_row / dst_row bytes apart.  Of the strides that
+ * are written each spans what the smaller ones do, so that nothing overlaps.  lengths (device, [batch], or NULL): of the
  * units of item b only the first lengths[b] move; what lies behind them is neither read nor written.
  */
 typedef struct {

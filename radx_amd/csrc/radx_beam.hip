@@ -10,6 +10,7 @@
 #include <stdint.h>
 #include <string.h>
 
+#include <algorithm>
 #include <new>
 
 #include "engine_host.h"
@@ -681,7 +682,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
     auto& lists = lds.slice.lists;
     __shared__ uint32_t is_last;
     __shared__ uint64_t block_kth;
-    __shared__ __attribute__((aligned(16))) uint32_t bins[kBins];
+    __shared__ __attribute__((aligned(16))) uint32_t bins[kBins], end_bins[kBins];  // of the first tile, of the lists
     __shared__ uint32_t listed[kWaves], wave_top[kWaves], some_count;
     __shared__ float wave_ref[kWaves];
     __shared__ double wave_total[kWaves];
@@ -766,6 +767,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
             const float high = wave_max(most);
             if (lane == 0) wave_top[wave] = ordered(high);
             bins[threadIdx.x] = bins[threadIdx.x + kThreads] = 0;
+            end_bins[threadIdx.x] = end_bins[threadIdx.x + kThreads] = 0;
             __syncthreads();
             const uint32_t o = max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3]));
 #pragma unroll
@@ -858,7 +860,6 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
 
     const double total = wave_sum(sum);
     pad_list(list, n);
-    bins[threadIdx.x] = bins[threadIdx.x + kThreads] = 0;
     if (lane == 0) {
         listed[wave] = n;
         wave_ref[wave] = ref;
@@ -879,10 +880,10 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
         // many more than k: first those that are near enough to the largest, by their counts
         uint64_t* const some = reinterpret_cast<uint64_t*>(lds.slice.queue);
         const uint32_t o = ordered(m);
-        for (uint32_t i = lane; i < n; i += 64) atomicAdd(&bins[bin_of(o - static_cast<uint32_t>(list[i] >> 32))], 1u);
+        for (uint32_t i = lane; i < n; i += 64) atomicAdd(&end_bins[bin_of(o - static_cast<uint32_t>(list[i] >> 32))], 1u);
         if (threadIdx.x == 0) some_count = 0;
         __syncthreads();
-        const uint32_t upto = bin_with(bins, k);
+        const uint32_t upto = bin_with(end_bins, k);
         for (uint32_t i = lane; i < n; i += 64)
             if (bin_of(o - static_cast<uint32_t>(list[i] >> 32)) <= upto) some[atomicAdd(&some_count, 1u)] = list[i];
         __syncthreads();
@@ -1247,6 +1248,19 @@ bool overlap(const void* p, uint64_t p_bytes, const void* q, uint64_t q_bytes) {
     return p && q && a < b + q_bytes && b < a + p_bytes;
 }
 
+// Whether each stride of the rows that are written spans all that the smaller ones do, so that no byte is written twice.
+bool nested(const radx_hip_beam_state& t, uint64_t rows) {
+    struct { uint64_t count, stride; } dims[3] = {{rows, t.dst_row}, {t.outer[0], t.dst_outer[0]}, {t.outer[1], t.dst_outer[1]}};
+    std::sort(dims, dims + 3, [](const auto& p, const auto& q) { return p.stride < q.stride; });
+    uint64_t extent = t.units * t.unit_bytes;
+    for (const auto& d : dims) {
+        if (d.count <= 1) continue;
+        if (d.stride < extent) return false;
+        extent += (d.count - 1) * d.stride;
+    }
+    return true;
+}
+
 // How a state's rows go to workgroups: threads a piece gets (a power of two, 16 bytes a thread), the parts of a
 // longer piece, and workgroups a batch item.
 struct RowCut {
@@ -1300,7 +1314,8 @@ int radx_hip_beam_create(int device, uint32_t max_batch, uint32_t max_beams, uin
     h->max_k = max_k;
     const hipError_t e = hipMalloc(reinterpret_cast<void**>(&h->scratch), radx_hip_beam_scratch_bytes(max_batch, max_beams, max_vocab, max_k));
     if (e != hipSuccess) { delete h; return fail(e, "hipMalloc(scratch)"); }
-    const hipError_t z = hipMemset(h->scratch, 0, arrived_bytes(max_batch));
+    hipError_t z = hipMemset(h->scratch, 0, arrived_bytes(max_batch));
+    if (z == hipSuccess) z = hipStreamSynchronize(nullptr);  // other streams do not wait for the null stream
     if (z != hipSuccess) { (void)hipFree(h->scratch); delete h; return fail(z, "hipMemset(scratch)"); }
     *out = h;
     return 0;
@@ -1429,6 +1444,7 @@ int radx_hip_beam_reorder(const radx_hip_beam_state* states, uint32_t n_states, 
         const bool same = t.src == t.dst;
         if (same && (t.src_row != t.dst_row || src_beams != dst_beams || t.src_outer[0] != t.dst_outer[0] || t.src_outer[1] != t.dst_outer[1]))
             return bad_arg("a state in place has two layouts");
+        if (!nested(t, static_cast<uint64_t>(batch) * dst_beams)) return bad_arg("a state's rows and pieces overlap");
         if (!same && overlap(t.src, (static_cast<uint64_t>(batch) * src_beams - 1) * t.src_row + reach[0], t.dst,
                              (static_cast<uint64_t>(batch) * dst_beams - 1) * t.dst_row + reach[1]))
             return bad_arg("a state's source and destination overlap");

@@ -96,6 +96,9 @@ def test_struct_formats_are_the_headers(tmp_path):
     (dict(dst=BASE + 4096), "source and destination overlap"), (dict(dst=BASE + 8 * 4096 - 1), "source and destination overlap"),
     (dict(units=1 << 41), "too long"), (dict(units=1 << 30, src_row=1 << 37, dst_row=1 << 37), "too long for one call"), (dict(unit_bytes=1 << 30, units=1 << 30), "too long"), (dict(src_row=1 << 41, dst_row=1 << 41), "out of range"),
     (dict(outer=(1 << 13, 1 << 12)), "pieces"), (dict(outer=(2, 1), src_outer=(100, 0), dst_outer=(100, 0)), "pieces overlap"),
+    (dict(outer=(2, 1), src_outer=(4096, 0), dst_outer=(4096, 0)), "rows and pieces overlap"),
+    (dict(outer=(2, 1), src_outer=(6144, 0), dst_outer=(6144, 0)), "rows and pieces overlap"),
+    (dict(outer=(3, 2), src_outer=(4096, 8192), dst_outer=(4096, 8192), src_row=1 << 16, dst_row=1 << 16), "rows and pieces overlap"),
     (dict(outer=(2, 1), src_outer=(1 << 41, 0), dst_outer=(1 << 41, 0)), "out of range"),
     (dict(outer=(2, 1), src_outer=(8192, 0), dst_outer=(4096, 0)), "two layouts"),
 ])

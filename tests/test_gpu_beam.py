@@ -335,6 +335,31 @@ def test_select_finished_beams(device, flag):
     sel.close()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [300, 40001])
+def test_select_subnormal_logits(device, dtype, vocab):
+    """Numbers below the type's normal ones, and zeros of both signs, which are one value.  Scores are given and cum is
+    0, so every one is exact."""
+    import torch
+    import radx_amd
+    k = 20
+    rng = np.random.default_rng(vocab)
+    step = float(torch.finfo(torch_dtype(dtype)).smallest_normal) * 2.0 ** -7  # a number of all three types
+    n = rng.integers(-100, 5, (2, vocab)).astype(np.float64)
+    n[1] = np.minimum(n[1], -0.0)  # the second beam has zeros of both signs at the top
+    n[1, ::3][n[1, ::3] == 0] = 0.0
+    logits = torch.from_numpy(n * step).to(torch_dtype(dtype))
+    x = logits.double().numpy().reshape(1, 2, vocab)
+    assert np.array_equal(x.reshape(2, vocab), n * step)
+    sel = radx_amd.BeamSelector(1, 2, vocab, k)
+    cum = np.zeros((1, 2), np.float32)
+    got = run_select(sel, logits.to(device), on(cum, device), k, normalize=False)
+    want = plain_best(plain_scores(x, cum, normalize=False) + 0.0, x, k)
+    assert np.array_equal(got[0], want[0].astype(np.float32))
+    assert np.array_equal(got[1], want[1]) and np.array_equal(got[2], want[2])
+    sel.close()
+
+
 def test_select_extreme_logits(device):
     """Float32 logits over the type's whole range, and cum scores far apart."""
     import torch
@@ -681,6 +706,9 @@ def test_reorder_refuses_tensors(device):
         radx_amd.beam_reorder(wide[:8], p, into=wide[1:])
     with pytest.raises(radx_amd.RadxError, match="written twice"):
         radx_amd.beam_reorder([s, s], p)
+    line = torch.zeros(100, device=device)
+    with pytest.raises(radx_amd.RadxError, match="rows and pieces overlap"):
+        radx_amd.beam_reorder(line.as_strided((8, 3, 2), (4, 4, 1)), p)
 
 
 # ---------------------------------------------------------------------------------------------
