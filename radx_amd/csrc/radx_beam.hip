@@ -252,6 +252,10 @@ struct SliceInfo {
     uint32_t unused;
 };
 
+// Counters are lines of their own: slices of other items that count in the same line cost more than all of an item's
+// (4 x 4 x 131072: 12.2 us a call with one line for all, 10.3 so).
+constexpr uint32_t kCounterWords = 32;
+
 struct SelectArgs {
     const void* logits;
     int64_t row_stride;         // elements
@@ -267,7 +271,7 @@ struct SelectArgs {
     uint32_t merge_parts_log2;  // threads that the join gives a list
     SliceInfo* info;            // [row][slice]
     uint64_t* best;             // [row][slice][k], best first: ordered logit, then ~token; 0: none
-    uint32_t* arrived;          // [batch]: slices of an item that are done; 0 between calls
+    uint32_t* arrived;          // [batch][kCounterWords], the first of each: slices of an item that are done; 0 between calls
     float* scores;
     int32_t* parents;
     int32_t* tokens;
@@ -284,7 +288,7 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 // Within a beam that is the slices' own order.
 constexpr uint32_t kMergeStage = 512;      // entries that are ranked at once; more than k only by ties and the bins' width
 constexpr uint32_t kMergeThreads = 1024;  // of the join as a kernel of its own
-constexpr uint32_t kHeld = 2;             // entries a thread of it fetches ahead, where that is all
+constexpr uint32_t kHeld = 2;             // entries of its first list that a thread fetches ahead
 
 struct Entry {
     uint64_t score;  // ordered64
@@ -364,11 +368,23 @@ struct MergeLds {
     uint32_t staged;
 };
 
-// A list has merge_parts threads, and a thread every merge_parts-th entry of it.  HELD: a thread has one list at most,
-// and at most so many entries of it, which it fetches ahead.  0: any number of lists.
-template <uint32_t THREADS, uint32_t HELD>
+// What the slices of a launch hand to the one that joins them goes past the XCDs' L2s: stores of agent scope write
+// through, and loads of that scope read behind them, so no L2 has to be written back or invalidated whole (8 x 4 x 32000, a
+// call: 11.4 us with a release and an acquire, 10.5 so).
+template <bool THROUGH, typename T>
+__device__ __forceinline__ void put(T* p, T v) {
+    if (THROUGH) __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    else *p = v;
+}
+template <bool THROUGH, typename T>
+__device__ __forceinline__ T got(const T* p) {
+    return THROUGH ? __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : *p;
+}
+
+// A list has merge_parts threads, and a thread every merge_parts-th entry of it.  Of its first list a thread fetches kHeld
+// entries ahead; ALL: that is all there is, otherwise it may have more entries, and more lists.
+template <uint32_t THREADS, bool ALL, bool THROUGH>
 __device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, MergeLds& lds) {
-    constexpr bool kAhead = HELD > 0;
     RowBase* const base = lds.base;
     Entry* const stage = lds.stage;
     uint32_t& staged = lds.staged;
@@ -379,13 +395,11 @@ __device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, M
     const uint32_t parts = 1u << a.merge_parts_log2, part = threadIdx.x & (parts - 1u);
     const uint32_t first_list = threadIdx.x >> a.merge_parts_log2, list_step = THREADS >> a.merge_parts_log2;
 
-    uint64_t held[kAhead ? HELD : 1];
-    if (kAhead) {
+    uint64_t held[kHeld];
 #pragma unroll
-        for (uint32_t r = 0; r < HELD; ++r) {
-            const uint32_t j = part + (r << a.merge_parts_log2);
-            held[r] = first_list < lists && j < a.k ? best[first_list * a.k + j] : 0;
-        }
+    for (uint32_t r = 0; r < kHeld; ++r) {
+        const uint32_t j = part + (r << a.merge_parts_log2);
+        held[r] = first_list < lists && j < a.k ? got<THROUGH>(best + first_list * a.k + j) : 0;
     }
     if (threadIdx.x == 0) staged = 0;
     for (uint32_t i = threadIdx.x; i < kBins; i += THREADS) lds.bins[0][i] = lds.bins[1][i] = 0;
@@ -402,16 +416,16 @@ __device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, M
         const SliceInfo* mine = info + beam * a.slices;
         // the first slice of every lane is fetched whole before any is looked at; most rows have no more
         const bool some = first < a.slices;
-        const float m0 = some ? mine[first].max : -INFINITY;
-        const double s0 = some ? mine[first].sum : 0.0;
+        const float m0 = some ? got<THROUGH>(&mine[first].max) : -INFINITY;
+        const double s0 = some ? got<THROUGH>(&mine[first].sum) : 0.0;
         float m = m0;
-        for (uint32_t s = first + group; s < a.slices; s += group) m = fmaxf(m, mine[s].max);
+        for (uint32_t s = first + group; s < a.slices; s += group) m = fmaxf(m, got<THROUGH>(&mine[s].max));
         for (uint32_t o = group >> 1; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
         auto scaled = [&](float ms, double p) {
             return ms > -INFINITY || !(p == 0.0) ? p * exp(static_cast<double>(ms) - static_cast<double>(m)) : 0.0;
         };
         double sum = scaled(m0, s0);
-        for (uint32_t s = first + group; s < a.slices; s += group) sum += scaled(mine[s].max, mine[s].sum);
+        for (uint32_t s = first + group; s < a.slices; s += group) sum += scaled(got<THROUGH>(&mine[s].max), got<THROUGH>(&mine[s].sum));
         for (uint32_t o = group >> 1; o; o >>= 1) sum += __shfl_xor(sum, o);
         // a NaN or +inf among the allowed logits has made the sum a NaN
         const bool live = !ended && finite(cum) && finite(m) && sum > 0.0 && sum < INFINITY;
@@ -438,20 +452,24 @@ __device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, M
         const uint32_t beam = divided(l, a.slices, a.slices_inverse);
         const RowBase r = base[beam];
         if (r.cum == -INFINITY) return;
-        if (kAhead) {
+        uint32_t from = part;
+        if (ALL || l == first_list) {
+            bool more = true;
 #pragma unroll
-            for (uint32_t i = 0; i < HELD; ++i) {
+            for (uint32_t i = 0; i < kHeld; ++i) {
                 const uint32_t bin = held[i] && part + (i << a.merge_parts_log2) < most_of_it ? bin_of(top, score_of(r, held[i])) : kBins;
-                if (bin <= last) f(held[i], beam, bin);
-                if (!__any(bin <= last)) break;
+                more = bin <= last;
+                if (more) f(held[i], beam, bin);
+                if (!__any(more)) break;
             }
-        } else {
-            for (uint32_t j = part; j < most_of_it; j += parts) {
-                const uint64_t key = best[static_cast<size_t>(l) * a.k + j];
-                const uint32_t bin = key ? bin_of(top, score_of(r, key)) : kBins;
-                if (bin > last) break;
-                f(key, beam, bin);
-            }
+            if (ALL || !more) return;
+            from += kHeld << a.merge_parts_log2;
+        }
+        for (uint32_t j = from; j < most_of_it; j += parts) {
+            const uint64_t key = got<THROUGH>(best + static_cast<size_t>(l) * a.k + j);
+            const uint32_t bin = key ? bin_of(top, score_of(r, key)) : kBins;
+            if (bin > last) break;
+            f(key, beam, bin);
         }
     };
     auto in_lists = [&](uint32_t last, uint32_t most_of_it, auto&& f) {
@@ -492,7 +510,7 @@ __device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, M
             const uint32_t now = min(step, lists - l0) * a.k;
             for (uint32_t i = threadIdx.x; i < now; i += THREADS) {
                 const uint32_t l = l0 + divided(i, a.k, a.k_inverse), beam = divided(l, a.slices, a.slices_inverse);
-                const uint64_t key = best[static_cast<size_t>(l0) * a.k + i];
+                const uint64_t key = got<THROUGH>(best + static_cast<size_t>(l0) * a.k + i);
                 if (!key || base[beam].cum == -INFINITY || bin_of(top, score_of(base[beam], key)) > upto) continue;
                 const Entry e = entry_of(base[beam], beam, key);
                 if (n_kept == a.k && !better(e, kept[a.k - 1])) continue;
@@ -522,10 +540,10 @@ __device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, M
     }
 }
 
-template <uint32_t HELD>
+template <bool ALL>
 __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(SelectArgs a) {
     __shared__ __attribute__((aligned(16))) MergeLds lds;
-    merge_item<kMergeThreads, HELD>(a, blockIdx.x, lds);
+    merge_item<kMergeThreads, ALL, false>(a, blockIdx.x, lds);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -696,8 +714,8 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
     if (!finite(a.cum[row]) || (a.finished && a.finished[row])) {
         // nothing is looked up in a row that offers nothing by its logits
         if (threadIdx.x == 0) {
-            info->sum = 0.0;
-            info->max = -INFINITY;
+            put<JOINED>(&info->sum, 0.0);
+            put<JOINED>(&info->max, -INFINITY);
         }
         if (JOINED) goto done;
         return;
@@ -874,7 +892,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
     if (all <= 2 * k) {
         for (uint32_t i = lane; i < n; i += 64) {
             const uint32_t rank = larger(lists, has, list[i]);
-            if (rank < k) best[rank] = list[i];
+            if (rank < k) put<JOINED>(best + rank, list[i]);
         }
     } else {
         // many more than k: first those that are near enough to the largest, by their counts
@@ -898,10 +916,10 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e) rank += j + e < count && other[e] > key;
             }
-            if (rank < k) best[rank] = key;
+            if (rank < k) put<JOINED>(best + rank, key);
         }
     }
-    for (uint32_t i = all + threadIdx.x; i < k; i += kThreads) best[i] = 0;
+    for (uint32_t i = all + threadIdx.x; i < k; i += kThreads) put<JOINED>(best + i, uint64_t{0});
     if (wave == 0) {
         double s = 0.0;
         if (lane < kWaves) {
@@ -912,27 +930,26 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
         s += __shfl_xor(s, 1);
         s += __shfl_xor(s, 2);
         if (lane == 0) {
-            info->sum = s;
-            info->max = m;
+            put<JOINED>(&info->sum, s);
+            put<JOINED>(&info->max, m);
         }
     }
     }
 done:
     if (!JOINED) return;
     const uint32_t item = row / a.beams, slices = a.beams * a.slices;
-    // every wave's stores have reached the XCD's L2 (a barrier alone does not wait for them) before one thread releases
-    // that L2 to whichever workgroup comes last, on whatever XCD; a release by each wave costs 0.9 us, this 0.2
+    // every wave's stores have gone through to where all XCDs see them (a barrier alone does not wait for that) before
+    // one thread counts the slice, and whichever workgroup comes last, on whatever XCD, reads them there
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) {
-        const uint32_t before = __hip_atomic_fetch_add(&a.arrived[item], 1u, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_AGENT);
+        const uint32_t before = __hip_atomic_fetch_add(&a.arrived[item * kCounterWords], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         is_last = before + 1 == slices;
-        if (before + 1 == slices) a.arrived[item] = 0;  // for the next call on the stream
+        if (before + 1 == slices) a.arrived[item * kCounterWords] = 0;  // for the next call on the stream
     }
     __syncthreads();
     if (!is_last) return;
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-    merge_item<kThreads, kHeld>(a, item, lds.merge);
+    merge_item<kThreads, false, true>(a, item, lds.merge);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1204,10 +1221,13 @@ namespace {
 // 131072, a call: 34 us at 1024 slices, 46 at 768, 39 at 1536, 37 at 2048).
 constexpr uint64_t kSlicesWanted = 1024;
 
-// Calls of at most this many slices, one a CU, are one launch: the last slice of an item joins its item.  That saves the
-// second launch (1 x 4 x 32000: 11.5 us a call as two, 9.9 as one) but makes every slice wait for its stores and
-// a counter, which costs more than it saves once the workgroups share CUs (16 x 8 x 65536: 15 us as two, 22 as one).
-constexpr uint32_t kJoinedSlices = 256;
+// Calls within these limits are one launch: the last slice of an item joins its item.  Measured, a call as one launch
+// against two (bfloat16): 1 x 8 x 65536, k = 4: 9.6 against 10.1 us; 16 x 8 x 65536, k = 16: 14.2, 15.4; 500 x 2 x 32000: 21.9,
+// 25.4; 64 x 8 x 131072, k = 16: 35, 36.5.  Not more slices an item, which all count in one word (1 x 12 x 131072,
+// 192 of them: 11.6, 10.6; 1024: 32, 18), nor more entries or places than the join's 256 threads (the other join has
+// 1024) are quick with (1 x 2 x 131072, k = 128: 21.5, 17.4), nor more slices in all than the CUs hold at once (2000 x 8 x
+// 32000: 248, 215).
+constexpr uint32_t kJoinedLists = 128, kJoinedEntries = 4096, kJoinedK = 64;
 
 struct Cut {
     uint32_t tiles_per_slice, slices;
@@ -1225,7 +1245,8 @@ uint64_t most_slices(uint64_t rows, uint64_t vocab) {
     const uint64_t all = rows * tiles;
     return all < kSlicesWanted + rows ? all : kSlicesWanted + rows;
 }
-uint64_t arrived_bytes(uint64_t batch) { return (batch * 4 + 255) & ~255ull; }
+// Counters for the items of calls that are one launch: such a call has kSlicesWanted slices at most.
+uint64_t arrived_bytes(uint64_t batch) { return (batch < kSlicesWanted ? batch : kSlicesWanted) * kCounterWords * 4; }
 uint64_t scratch_of(uint64_t batch, uint64_t beams, uint64_t vocab, uint64_t k) {
     return arrived_bytes(batch) + most_slices(batch * beams, vocab) * (sizeof(SliceInfo) + k * 8);
 }
@@ -1400,7 +1421,7 @@ int radx_hip_beam_select(radx_hip_beam* h, const radx_hip_beam_select_args* s, v
     };
     auto held = [&](uint32_t log2) { return (a.k + (1u << log2) - 1) >> log2; };
     a.merge_parts_log2 = parts_log2(kThreads);
-    const bool joined = n_rows * a.slices <= kJoinedSlices && lists <= kThreads && held(a.merge_parts_log2) <= kHeld;
+    const bool joined = n_rows * a.slices <= kSlicesWanted && lists <= kJoinedLists && lists * a.k <= kJoinedEntries && a.k <= kJoinedK;
     if (!joined) a.merge_parts_log2 = parts_log2(kMergeThreads);
     if (s->dtype == RADX_HIP_F32) launch_slices<float>(a, n_rows, joined, st);
     else if (s->dtype == RADX_HIP_BF16) launch_slices<BF16>(a, n_rows, joined, st);
@@ -1408,8 +1429,8 @@ int radx_hip_beam_select(radx_hip_beam* h, const radx_hip_beam_select_args* s, v
     RADX_TRY(hipGetLastError());
     if (joined) return 0;
     const dim3 items(s->batch), block(kMergeThreads);
-    if (lists <= kMergeThreads && held(a.merge_parts_log2) <= kHeld) hipLaunchKernelGGL(beam_merge_kernel<kHeld>, items, block, 0, st, a);
-    else hipLaunchKernelGGL(beam_merge_kernel<0>, items, block, 0, st, a);
+    if (lists <= kMergeThreads && held(a.merge_parts_log2) <= kHeld) hipLaunchKernelGGL(beam_merge_kernel<true>, items, block, 0, st, a);
+    else hipLaunchKernelGGL(beam_merge_kernel<false>, items, block, 0, st, a);
     RADX_TRY(hipGetLastError());
     return 0;
 }

@@ -116,7 +116,7 @@ def check_best(got, scores, x, k, vocab, normalize=True):
 
 SHAPES = [(1, 1, 1, 1), (1, 1, 5, 8), (2, 3, 7, 4), (1, 4, 31, 8), (3, 2, 32, 4), (2, 5, 33, 10), (1, 2, 255, 16), (1, 64, 100, 128),
           (2, 4, 1023, 8), (1, 4, 4096, 8), (1, 3, 4097, 6), (2, 2, 8192, 4), (2, 2, 8193, 33), (1, 5, 20011, 10), (3, 8, 50001, 16),
-          (1, 4, 131072, 64), (5, 1, 70001, 1), (1, 7, 40003, 128)]
+          (1, 4, 131072, 64), (5, 1, 70001, 1), (1, 7, 40003, 128), (300, 3, 2001, 4), (4, 16, 33000, 40)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
