@@ -158,6 +158,7 @@ template <> struct Vec<_Float16> : Half16 {
         for (int i = 0; i < 4; ++i) {
             f[2 * i] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[i])));
             f[2 * i + 1] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[i] >> 16)));
+            asm("" : "+v"(f[2 * i]), "+v"(f[2 * i + 1]));  // or the halves stay in registers beside them, and these spill
         }
     }
     static __device__ __forceinline__ uint4 pack(const float* f) {  // the values are float16's: nothing is rounded
@@ -680,9 +681,10 @@ __device__ __forceinline__ uint32_t larger(const uint64_t (*lists)[kWaveList + 8
 
 // Candidates are the elements that reach a threshold which k elements are known to reach: in the first tile
 // one that k of its 1024 vectors' maxima reach (few more do, by their counts), then the k-th best of that
-// tile.  Every wave collects its own in a list, so nothing waits inside the loop over the other tiles.  The few
-// vectors that hold a candidate go through a queue, where a wave tests 64 of their elements at a time: a
-// test and a branch for every element of a tile took 15 of 40 us (64 x 8 x 131072 bfloat16, k = 16).
+// tile, in long slices later on one by the counts of all candidates.  Every wave collects its own in a list, so
+// nothing waits inside the loop over the other tiles.  The few vectors that hold a candidate go through a queue, where a
+// wave tests 64 of their elements at a time: a test and a branch for every element of a tile took 15 of 40 us
+// (64 x 8 x 131072 bfloat16, k = 16).
 // JOINED: the workgroup that finishes an item's last slice joins them.
 template <typename T, bool MASKED, bool JOINED>
 __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
@@ -700,7 +702,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
     auto& lists = lds.slice.lists;
     __shared__ uint32_t is_last;
     __shared__ uint64_t block_kth;
-    __shared__ __attribute__((aligned(16))) uint32_t bins[kBins], end_bins[kBins];  // of the first tile, of the lists
+    __shared__ __attribute__((aligned(16))) uint32_t bins[kBins], end_bins[kBins], seen[kBins];  // of the first tile, of the lists, of candidates
     __shared__ uint32_t listed[kWaves], wave_top[kWaves], some_count;
     __shared__ float wave_ref[kWaves];
     __shared__ double wave_total[kWaves];
@@ -727,6 +729,10 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
     const uint32_t last = min(a.vocab, first + a.tiles_per_slice * kTile);
     const uint32_t mine = wave * (kTile / kWaves) + lane * V;
 
+    // candidates are counted by their distance below the first tile's maximum, so that the threshold rises with the tiles:
+    // after n of them a tile has k / n candidates, not k (64 x 8 x 131072 bfloat16, a call: k = 16 36.7 -> 33.4 us, 64 50.5 -> 41.0).  Not
+    // in slices of few tiles (64 x 4 x 65536 float32, four tiles: 20.1 -> 20.9).
+    const bool counted = last - first > 4 * kTile;
     uint64_t* list = lists[wave];
     uint4* queue = lds.slice.queue[wave];
     uint32_t* queue_token = lds.slice.queue_token[wave];
@@ -735,6 +741,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
     float thr = -FLT_MAX;        // and so an element: the logit of `reach`
     double sum = 0.0;            // this lane's share, relative to ref
     float ref = -INFINITY;       // the wave's maximum so far (the workgroup's, in the first tile)
+    uint32_t high = 0;           // the first tile's maximum, ordered
 
     // the queue's vectors in order of their tokens, 64 elements at a time; all of them, or whole rounds only
     constexpr uint32_t kRound = 64 / V;
@@ -782,17 +789,19 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
             most = fmaxf(most, top[j]);
         }
         if (tile == first) {
-            const float high = wave_max(most);
-            if (lane == 0) wave_top[wave] = ordered(high);
+            const float wave_high = wave_max(most);
+            if (lane == 0) wave_top[wave] = ordered(wave_high);
             bins[threadIdx.x] = bins[threadIdx.x + kThreads] = 0;
             end_bins[threadIdx.x] = end_bins[threadIdx.x + kThreads] = 0;
+            if (counted) seen[threadIdx.x] = seen[threadIdx.x + kThreads] = 0;
             __syncthreads();
             const uint32_t o = max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3]));
 #pragma unroll
             for (int j = 0; j < kVecs; ++j)
                 if (top[j] >= thr) atomicAdd(&bins[bin_of(o - ordered(top[j]))], 1u);
             __syncthreads();
-            ref = uniform(from_ordered(o));
+            high = uniform(o);
+            ref = from_ordered(high);
             const uint32_t within = end_of_bin(bin_with(bins, k));
             if (o > kLowestFinite && o - kLowestFinite > within) {
                 thr = uniform(from_ordered(o - within));
@@ -847,6 +856,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
                     const uint32_t slot = q + lanes_before(who[j]);
                     queue[slot] = Vec<T>::pack(f + j * V);
                     queue_token[slot] = tile + mine + j * 64 * V;
+                    if (counted && tile != first) atomicAdd(&seen[bin_of(high - min(high, ordered(top[j])))], 1u);
                 }
                 q += __popcll(who[j]);
             }
@@ -857,14 +867,26 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
             reach = ((reach >> 32) + 1) << 32;
             thr = from_ordered(static_cast<uint32_t>(reach >> 32));
         }
+        // after the second tile, the fourth, the eighth: what other waves have not counted yet leaves the threshold lower
+        const uint32_t before = (tile - first) / kTile;
+        if (counted && before && (before & (before + 1)) == 0 && !final_tile) {
+            const uint32_t within = end_of_bin(bin_with(seen, k));
+            if (high > within && high - within > static_cast<uint32_t>(reach >> 32)) {
+                reach = static_cast<uint64_t>(uniform(high - within)) << 32;
+                thr = from_ordered(static_cast<uint32_t>(reach >> 32));
+            }
+        }
         if (tile == first && tile + kTile < last) {
             if (threadIdx.x == 0) block_kth = 0;
             if (lane == 0) listed[wave] = n;
             pad_list(list, n);
             __syncthreads();
             const uint32_t has[kWaves] = {uniform(listed[0]), uniform(listed[1]), uniform(listed[2]), uniform(listed[3])};
-            for (uint32_t i = lane; i < n; i += 64)
-                if (larger(lists, has, list[i]) == k - 1) block_kth = list[i];
+            for (uint32_t i = lane; i < n; i += 64) {
+                const uint32_t rank = larger(lists, has, list[i]);
+                if (counted && rank < k) atomicAdd(&seen[bin_of(high - static_cast<uint32_t>(list[i] >> 32))], 1u);
+                if (rank == k - 1) block_kth = list[i];
+            }
             __syncthreads();
             const uint64_t beyond = ((uniform(block_kth) >> 32) + 1) << 32;
             if (block_kth && beyond > reach) {

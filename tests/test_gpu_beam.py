@@ -417,6 +417,43 @@ def test_select_lists_and_queues(device, kind, dtype, k):
     sel.close()
 
 
+@pytest.mark.parametrize("kind", ["normal", "rising", "falling", "few values", "late", "first tile empty", "under a mask"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k", [4, 64, 128])
+def test_select_long_slices(device, kind, dtype, k):
+    """So many rows that one workgroup takes a whole one of ten tiles (of 4096 elements, 8192 of the 16-bit types), whose
+    threshold rises on the way.  Three items are compared."""
+    import torch
+    import radx_amd
+    batch, beams, tile = 256, 4, 4096 if dtype == "f32" else 8192
+    vocab = 9 * tile + 77
+    g = torch.Generator(device=device).manual_seed(k)
+    x = torch.randn((batch * beams, vocab), generator=g, device=device)
+    token = torch.arange(vocab, device=device)
+    allowed = None
+    if kind == "rising":
+        x = x * 1e-2 + token / vocab * 30.0
+    elif kind == "falling":
+        x = x * 1e-2 - token / vocab * 30.0
+    elif kind == "few values":
+        x = (x * 2).round() * 0.5
+    elif kind == "late":
+        x[:, 7 * tile:8 * tile:5] += 8.0
+    elif kind == "first tile empty":
+        x[:, :tile] = -math.inf
+    elif kind == "under a mask":
+        allowed = np.random.default_rng(k).random((1, vocab)) < 0.02
+    x = x.to(torch_dtype(dtype))
+    cum = -torch.rand((batch, beams), generator=g, device=device)
+    sel = radx_amd.BeamSelector(batch, beams, vocab, k)
+    got = run_select(sel, x, cum, k, allowed=None if allowed is None else on(words_of(allowed), device))
+    items = [0, 100, 255]
+    xv = x.view(batch, beams, vocab)[items].double().cpu().numpy()
+    full = None if allowed is None else np.broadcast_to(allowed, xv.shape)
+    check_best([part[items] for part in got], plain_scores(xv, cum.cpu().numpy()[items], allowed=full), xv, k, vocab)
+    sel.close()
+
+
 def test_select_past_32_bits(device):
     """Rows that begin more than 4 GiB into the logits."""
     import torch
