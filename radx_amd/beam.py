@@ -248,29 +248,29 @@ def beam_reorder(states, parents, into=None, lengths=None, length_dim=None, row_
     if batch == 0 or k == 0:
         return
     table, beams, address = [], None, capi.ADDRESSES.pack
-    like = packed = None
+    like_shape = like_strides = like_d_strides = like_dtype = packed = None
     for i, s in enumerate(states):
         if s.get_device() != dev:
             _on(s, "a state", dev)
-        has, strides = s.shape, s.stride()
-        d, d_strides = s, strides
+        has, strides, dtype = s.shape, s.stride(), s.dtype
+        at = d_at = s.data_ptr()
+        d_strides = strides
         if into is not None:
             d = into[i]
             _on(d, "into", dev)
             row = row_dim + len(has) if row_dim < 0 else row_dim
-            if d.dtype != s.dtype or d.shape != tuple(batch * k if n == row else size for n, size in enumerate(has)):
+            if d.dtype != dtype or d.shape != tuple(batch * k if n == row else size for n, size in enumerate(has)):
                 raise ValueError("into must have the states' dtypes and shapes, with batch * k rows")
-            d_strides = d.stride()
-        if like != (has, strides, d_strides, s.dtype):  # states are often alike
-            like = (has, strides, d_strides, s.dtype)
+            d_strides, d_at = d.stride(), d.data_ptr()
+        if has != like_shape or strides != like_strides or d_strides != like_d_strides or dtype is not like_dtype:  # they are often alike
+            like_shape, like_strides, like_d_strides, like_dtype = has, strides, d_strides, dtype
             rows, packed = _layout(has, strides, d_strides, s.element_size(), row_dim, length_dim, batch)
             if rows != beams:
                 if beams is not None:
                     raise ValueError("the states have different numbers of rows")
                 beams = rows
         if packed is not None:
-            table.append(address(s.data_ptr(), d.data_ptr()))
-            table.append(packed)
+            table += (address(at, d_at), packed)
     if not table or not beams:
         return
     code = capi.lib.radx_hip_beam_reorder(b"".join(table), len(table) // 2, parents_at, lengths_at, batch, beams, beams if into is None else k, k,
