@@ -243,7 +243,7 @@ __device__ __forceinline__ uint32_t reached_by(const uint32_t (&v)[N], uint32_t 
 // the sum are known, and the logits are read once.  A workgroup takes a slice of a row and leaves the
 // slice's maximum, its sum of exponentials relative to that maximum and its k best logits; another joins the
 // slices of an item.  What bounds it, large: reading, and the issue of about seven operations an element beside it
-// (64 x 8 x 131072 bfloat16, k = 16: 33 us for 134 MB, 4.1 TB/s; the loads and maxima alone take 26).  Small: the
+// (64 x 8 x 131072 bfloat16, k = 16: a call 33 us for 134 MB, 4.1 TB/s; the loads and maxima alone take 26).  Small: the
 // latency of the two phases (1 x 4 x 32000 float32: 10 us).
 // Exponentials are 32-bit, eight of them are added in 32 bits and from there on in 64; scores are 64-bit and rounded
 // once, so that the order of two candidates of different rows hangs on their rows' sums alone (about 1e-8).
@@ -729,9 +729,9 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
     const uint32_t last = min(a.vocab, first + a.tiles_per_slice * kTile);
     const uint32_t mine = wave * (kTile / kWaves) + lane * V;
 
-    // candidates are counted by their distance below the first tile's maximum, so that the threshold rises with the tiles:
-    // after n of them a tile has k / n candidates, not k (64 x 8 x 131072 bfloat16, a call: k = 16 36.7 -> 33.4 us, 64 50.5 -> 41.0).  Not
-    // in slices of few tiles (64 x 4 x 65536 float32, four tiles: 20.1 -> 20.9).
+    // candidates are counted by their distance below the first tile's maximum, so that the threshold rises with the
+    // tiles: after n of them a tile has k / n candidates, not k (64 x 8 x 131072 bfloat16, a call: k = 16 36.7 -> 33.3 us,
+    // k = 64 50.5 -> 41.0).  Not in slices of few tiles (64 x 4 x 65536 float32, four tiles: 20.1 -> 20.9).
     const bool counted = last - first > 4 * kTile;
     uint64_t* list = lists[wave];
     uint4* queue = lds.slice.queue[wave];
@@ -1240,7 +1240,7 @@ namespace {
 
 // Slices that the rows of a call are cut into: the workgroups that 256 CUs hold at once.  With more, every slice's first
 // threshold and last ranking weigh more, and so does the join; with fewer, CUs have too little in flight (64 x 8 x
-// 131072, a call: 34 us at 1024 slices, 46 at 768, 39 at 1536, 37 at 2048).
+// 131072, a call: 33 us at 1024 slices, 40 at 768, 39 at 1536, 40 at 2048).
 constexpr uint64_t kSlicesWanted = 1024;
 
 // Calls within these limits are one launch: the last slice of an item joins its item.  Measured, a call as one launch
