@@ -172,11 +172,17 @@ class BeamSelector:
 @functools.lru_cache(maxsize=4096)
 def _pieces(shape, src_strides, dst_strides, size, row_dim, length_dim):
     """The rows of a layout as radx_hip_beam_state counts them, strides in bytes:
-    (src_row, dst_row, src_outer, dst_outer, outer, unit_bytes, units)."""
+    (src_row, dst_row, src_outer, dst_outer, outer, unit_bytes, units).  The dimensions are taken in the order in which
+    they lie in the memory that is written, whatever their order in the tensor."""
     dims = [(n, s * size, d * size, i == length_dim) for i, (n, s, d) in enumerate(zip(shape, src_strides, dst_strides))
-            if i != row_dim and (n != 1 or i == length_dim)]
+            if i != row_dim and n != 1]
+    dims.sort(key=lambda dim: dim[2:0:-1], reverse=True)
     run, units = size, None
-    while dims and units is None and ((dims[-1][1] == run and dims[-1][2] == run) or (dims[-1][3] and dims[-1][0] == 1)):
+    if length_dim is not None and shape[length_dim] == 1:
+        units = 1  # the only position: all of the row or nothing
+        while dims and dims[-1][1] == run and dims[-1][2] == run:
+            run *= dims.pop()[0]
+    while dims and units is None and dims[-1][1] == run and dims[-1][2] == run:
         n, _, _, counted = dims.pop()
         if counted:
             units = n
@@ -225,9 +231,11 @@ def beam_reorder(states, parents, into=None, lengths=None, length_dim=None, row_
 
     Rows whose parent is < 0 or >= beams, and rows k.. of an item, are left as they were.  states: a tensor or a
     sequence of them, any dtypes and layouts of whole rows (up to two strided dimensions around contiguous
-    pieces); they must not share memory with each other.  into: as many tensors that get the rows instead (b * k + j),
-    apart from the states.  lengths: int32 [batch]; of dimension length_dim only the first lengths[b] positions
-    move, what lies behind is neither read nor written."""
+    pieces, in any order of the tensor's dimensions); they must not share memory with each other.  into: as many tensors
+    that get the rows instead (b * k + j), apart from the states.  lengths: int32 [batch]; of dimension length_dim only the
+    first lengths[b] positions move, what lies behind is neither read nor written.  The bytes of a position, and those of
+    the positions after it, must follow each other in memory (what a row has more than one of, such as heads, may lie
+    around them; a cache whose positions lie outside its rows has no lengths)."""
     states = (states,) if hasattr(states, "data_ptr") else tuple(states)
     if into is not None:
         into = (into,) if hasattr(into, "data_ptr") else tuple(into)
