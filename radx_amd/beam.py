@@ -5,7 +5,8 @@ include/radx_hip.h.  A decoding step is
     beam_reorder(states, parents)                               # their states to their places
 
 and after the last one beam_backtrace(tokens, parents) gives the sequences.  torch is used for device
-memory and streams only; the work happens in the library's kernels.  As for the sort, torch is imported before this
+memory and streams only; the work happens in the library's kernels, none of which has a gradient: results carry
+none, and tensors that a call writes count as modified in place.  As for the sort, torch is imported before this
 package: it brings a HIP runtime of its own, which the library then shares.
 """
 import ctypes
@@ -26,6 +27,8 @@ def _torch():
         empty_like = torch.empty_like
         # the handle alone, which a torch.cuda.Stream would cost a microsecond more for
         raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+        # tells autograd that tensors were written, so that a backward pass that still needs their old values raises
+        written = getattr(torch._C, "_increment_version", None) or torch.autograd.graph.increment_version
     _torch = lambda: names  # noqa: E731
     return names
 
@@ -137,8 +140,8 @@ class BeamSelector:
                 raise ValueError("end_token %d is outside the vocabulary" % end)
         if not 1 <= k <= capi.BEAM_MAX_K:
             raise ValueError("k must be 1..%d, got %d" % (capi.BEAM_MAX_K, k))
-        size = (batch, k)
-        if out is None:
+        size, given = (batch, k), out is not None
+        if not given:
             if stream is None:
                 out = self._outputs(T, cum, finished, size)
             else:
@@ -160,6 +163,8 @@ class BeamSelector:
         code = capi.lib.radx_hip_beam_select(self._h, args, _stream(stream, dev))
         if code:
             capi.check(code)
+        if given:
+            T.written(out)
         return out
 
     @staticmethod
@@ -285,6 +290,7 @@ def beam_reorder(states, parents, into=None, lengths=None, length_dim=None, row_
                                           _stream(stream, dev))
     if code:
         capi.check(code)
+    T.written(states if into is None else into)
 
 
 def beam_backtrace(tokens, parents, steps=None, out=None, stream=None):
@@ -318,4 +324,5 @@ def beam_backtrace(tokens, parents, steps=None, out=None, stream=None):
     code = capi.lib.radx_hip_beam_backtrace(tokens_at, parents_at, steps_at, total, batch, k, out.data_ptr(), stride, _stream(stream, dev))
     if code:
         capi.check(code)
+    T.written((out,))
     return out
