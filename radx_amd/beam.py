@@ -35,7 +35,11 @@ def _torch():
 
 def _stream(stream, index):
     """The handle of a stream, by default the device's current one."""
-    return getattr(stream, "cuda_stream", stream) if stream is not None else _torch().raw_stream(index)
+    if stream is None:
+        return _torch().raw_stream(index)
+    if getattr(stream, "device_index", index) != index:
+        raise ValueError("the stream is of cuda:%d, expected cuda:%d" % (stream.device_index, index))
+    return getattr(stream, "cuda_stream", stream)
 
 
 def _made_on(stream, index):
@@ -140,7 +144,7 @@ class BeamSelector:
                 raise ValueError("end_token %d is outside the vocabulary" % end)
         if not 1 <= k <= capi.BEAM_MAX_K:
             raise ValueError("k must be 1..%d, got %d" % (capi.BEAM_MAX_K, k))
-        size, given = (batch, k), out is not None
+        size, given, handle = (batch, k), out is not None, _stream(stream, dev)
         if not given:
             if stream is None:
                 out = self._outputs(T, cum, finished, size)
@@ -160,7 +164,7 @@ class BeamSelector:
                 ended_at = _plain(out[3], T.flags, size, "out finished", dev)
         args = capi.BEAM_SELECT_ARGS.pack(logits.data_ptr(), stride, cum_at, allowed_at, allowed_stride, finished_at, *at, ended_at,
                                           batch, beams, vocab, k, dtype, 1 if normalize else 0, end)
-        code = capi.lib.radx_hip_beam_select(self._h, args, _stream(stream, dev))
+        code = capi.lib.radx_hip_beam_select(self._h, args, handle)
         if code:
             capi.check(code)
         if given:
@@ -307,6 +311,7 @@ def beam_backtrace(tokens, parents, steps=None, out=None, stream=None):
     tokens_at = _plain(tokens, (T.i32,), shape, "tokens", dev)
     parents_at = _plain(parents, (T.i32,), shape, "parents", dev)
     steps_at = None if steps is None else _plain(steps, (T.i32,), (batch,), "steps", dev)
+    handle = _stream(stream, dev)
     if out is None:
         if stream is not None:
             with _made_on(stream, dev):
@@ -321,7 +326,7 @@ def beam_backtrace(tokens, parents, steps=None, out=None, stream=None):
     if total == 0 or batch == 0 or k == 0:
         return out
     stride = strides[1] if k > 1 else strides[0] if batch > 1 else total
-    code = capi.lib.radx_hip_beam_backtrace(tokens_at, parents_at, steps_at, total, batch, k, out.data_ptr(), stride, _stream(stream, dev))
+    code = capi.lib.radx_hip_beam_backtrace(tokens_at, parents_at, steps_at, total, batch, k, out.data_ptr(), stride, handle)
     if code:
         capi.check(code)
     T.written((out,))
