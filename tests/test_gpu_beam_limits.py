@@ -1,5 +1,8 @@
 """Beam search calls at the ends of what they take."""
+import numpy as np
 import pytest
+
+from test_gpu_beam import on
 
 pytestmark = pytest.mark.gpu
 
@@ -18,3 +21,68 @@ def test_streams_of_another_device_are_refused(device):
         with pytest.raises(ValueError, match="the stream is of"):
             call()
     sel.close()
+
+
+def test_select_of_the_most_items(device):
+    """2^20 items of four beams, which share a row of logits.  Numbers are small multiples of 1/64, so that scores are
+    exact, and tie between beams."""
+    import torch
+    import radx_amd
+    batch, beams, vocab, k = 1 << 20, 4, 10, 3
+    g = torch.Generator(device=device).manual_seed(1)
+    row = torch.randperm(vocab, generator=g, device=device).float().reshape(1, vocab) / 64
+    cum = -torch.randint(0, 30, (batch, beams), generator=g, device=device).float() / 64
+    sel = radx_amd.BeamSelector(batch, beams, vocab, k)
+    scores, parents, tokens = sel.select(row.expand(batch * beams, vocab), cum, k, normalize=False)
+    best, at = (cum.unsqueeze(2) + row).reshape(batch, beams * vocab).sort(dim=1, descending=True, stable=True)
+    assert torch.equal(scores, best[:, :k])
+    assert torch.equal(parents, (at[:, :k] // vocab).int()) and torch.equal(tokens, (at[:, :k] % vocab).int())
+    sel.close()
+
+
+def test_reorder_of_the_most_items(device):
+    import torch
+    import radx_amd
+    batch, beams, width = 65535, 3, 5
+    g = torch.Generator(device=device).manual_seed(2)
+    state = torch.randint(0, 1 << 30, (batch * beams, width), generator=g, device=device, dtype=torch.int32)
+    parents = torch.randint(-1, beams + 1, (batch, beams), generator=g, device=device, dtype=torch.int32)
+    place = torch.arange(beams, device=device)
+    source = torch.where((parents >= 0) & (parents < beams), parents.long(), place) + torch.arange(batch, device=device).unsqueeze(1) * beams
+    want = state[source.reshape(-1)]
+    radx_amd.beam_reorder(state, parents)
+    assert torch.equal(state, want)
+
+
+def test_backtrace_of_the_most_items(device):
+    import torch
+    import radx_amd
+    total, batch, k = 7, 65535, 4
+    g = torch.Generator(device=device).manual_seed(3)
+    tokens = torch.randint(0, 1 << 30, (total, batch, k), generator=g, device=device, dtype=torch.int32)
+    parents = torch.randint(0, k, (total, batch, k), generator=g, device=device, dtype=torch.int32)
+    steps = torch.randint(0, total + 1, (batch,), generator=g, device=device, dtype=torch.int32)
+    got = radx_amd.beam_backtrace(tokens, parents, steps=steps)
+    place = torch.arange(k, device=device).expand(batch, k)
+    for t in range(total - 1, -1, -1):
+        live = (t < steps).unsqueeze(1)
+        assert torch.equal(got[:, :, t], torch.where(live, tokens[t].gather(1, place), -1))
+        place = torch.where(live, parents[t].gather(1, place).long(), place)
+
+
+@pytest.mark.parametrize("ends", [None, (1 << 24) - 70000])
+def test_backtrace_of_the_most_steps(device, ends):
+    """Two beams whose places a step keeps or exchanges: the place at a step is the sum of the exchanges behind it."""
+    import radx_amd
+    total = (1 << 24) - 1
+    last = total if ends is None else ends
+    rng = np.random.default_rng(4)
+    change = rng.integers(0, 2, total, dtype=np.int32)
+    tokens = rng.integers(0, 1 << 30, (total, 1, 2), dtype=np.int32)
+    parents = np.stack([change, 1 - change], 1).reshape(total, 1, 2)
+    steps = None if ends is None else on(np.array([ends], np.int32), device)
+    got = radx_amd.beam_backtrace(on(tokens, device), on(parents, device), steps=steps).cpu().numpy()
+    behind = np.concatenate([np.bitwise_xor.accumulate(change[1:last][::-1])[::-1], [0]])
+    for j in range(2):
+        assert np.array_equal(got[0, j, :last], tokens[np.arange(last), 0, behind ^ j])
+        assert (got[0, j, last:] == -1).all()
