@@ -25,7 +25,8 @@ namespace radx {
         BeamSearch& operator=(const BeamSearch&) = delete;
         virtual ~BeamSearch() { (void)radx_hip_beam_destroy(beam); }
 
-        // Limits of the selections to come; the scratch of one of them in flight.
+        // Limits of the selections to come; the scratch of one of them in flight: calls on several command buffers' streams
+        // are put in order by the caller, or get an object each.
         virtual BeamSearch& initialize(const std::shared_ptr<Device>& device, uint32_t maxBatch, uint32_t maxBeams, uint32_t maxVocabulary,
                                        uint32_t maxPlaces) {
             radx_hip_beam* made = nullptr;

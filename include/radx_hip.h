@@ -282,7 +282,9 @@ size_t radx_hip_beam_scratch_bytes(uint32_t max_batch, uint32_t max_beams, uint3
 /*
  * Create the handle of selections of at most max_batch (1..2^20) items x max_beams (1..64) beams (2^22 rows) x max_vocab
  * (1..2^24) tokens, max_k (1..128) places, on HIP device `device`.  It owns the scratch of the call in flight: one
- * selection may be in flight per handle, also between two captured graphs.
+ * selection may be in flight per handle, also between two captured graphs, which it has to outlive.  Calls on several
+ * streams have to be put in order by the caller, or be given a handle each: selections that overlap on one handle get wrong
+ * results, and leave its counters so that later ones may, all without an error; such a handle is to be made anew.
  */
 int radx_hip_beam_create(int device, uint32_t max_batch, uint32_t max_beams, uint32_t max_vocab, uint32_t max_k,
                          radx_hip_beam** out);
@@ -295,7 +297,9 @@ int radx_hip_beam_destroy(radx_hip_beam* h);
  *   score(b, i, v) = cum[b][i] + logits[b * beams + i][v]                   (normalize == 0: log probabilities given)
  *
  * Compared in 64 bits and rounded to the float that scores[] gets; equal scores go to the lower beam, in a beam
- * to the larger logit, then to the lower token.
+ * to the larger logit, then to the lower token.  The softmax's sum is one of 32-bit exponentials: a row's log of it is within
+ * (3 ln vocab + 5) 2^-24 (ordinary rows: some 1e-8), by which the scores of all its tokens are off alike.  So the order
+ * within a beam is exact, and of two beams' tokens unless their scores are closer than twice that.
  *   allowed       bit v & 31 of word v >> 5 of a row: token v may be chosen.  The others count as -inf, in the
  *                 softmax too, whatever their logits hold.  allowed_stride: words between rows, 0 = one mask for all.
  *   finished      beams that have ended (bytes, 0 or not): such a beam offers end_token at its cum score and
@@ -332,7 +336,7 @@ int radx_hip_beam_select(radx_hip_beam* h, const radx_hip_beam_select_args* args
  * parents[batch][k] on the device, batch < 2^16, k <= 64; where a parent is < 0 or >= src_beams the row is left as it was.
  * In place (dst == src, same layout): rows are read and written as if all were read first, a row that stays
  * is not touched, rows k.. of an item stay.  Otherwise src and dst must not overlap.  The states of a call must
- * not share bytes with each other.
+ * not share bytes with each other, nor with parents or lengths.
  * A row is outer[0] x outer[1] pieces, src_outer[] / dst_outer[] bytes apart, of units x unit_bytes contiguous
  * bytes each (fewer than 64 GiB a row), at any alignment; rows are src_row / dst_row bytes apart.  Of the strides that
  * are written each spans what the smaller ones do, so that nothing overlaps.  lengths (device, [batch], or NULL): of the

@@ -71,7 +71,8 @@ def _plain(t, dtypes, shape, name, index):
 
 class BeamSelector:
     """One radx_hip_beam handle: the scratch of selections within these limits.  One selection may be in
-    flight per handle; use one handle per concurrent stream or graph."""
+    flight per handle; use one handle per concurrent stream or graph, or put the calls in order.  Selections that overlap on a
+    handle get wrong results, and later ones on it may, without an error; it has to outlive the graphs that captured it."""
 
     def __init__(self, max_batch, max_beams, max_vocab, max_k, device=0):
         self.device = device
@@ -98,7 +99,8 @@ class BeamSelector:
         log_softmax(logits), otherwise cum + logits.  allowed: int32 words [batch * beams or 1, ceil(vocab / 32)], bit
         v & 31 of word v >> 5 admits token v.  finished: bool or uint8 [batch, beams]; such a beam offers end_token
         at its own score.  Equal scores go to the lower beam, the larger logit, the lower token; places that are
-        left over get -inf, -1, -1.  out: the tensors to write, as returned."""
+        left over get -inf, -1, -1.  out: the tensors to write, as returned.  The order in a beam is exact, and
+        of different beams' tokens unless their scores are closer than twice what a sum's log may be off by, (3 ln vocab + 5) 2^-24."""
         T, dev = _torch(), self.device
         shape = cum.shape
         if len(shape) != 2:

@@ -243,12 +243,12 @@ __device__ __forceinline__ uint32_t reached_by(const uint32_t (&v)[N], uint32_t 
 // the sum are known, and the logits are read once.  A workgroup takes a slice of a row and leaves the
 // slice's maximum, its sum of exponentials relative to that maximum and its k best logits; another joins the
 // slices of an item.  What bounds it, large: reading, and the issue of about seven operations an element beside it
-// (64 x 8 x 131072 bfloat16, k = 16: a call 34.7 us for 134 MB, 3.9 TB/s; the loads and maxima alone take 26).  Small: the
+// (64 x 8 x 131072 bfloat16, k = 16: a call 34.9 us for 134 MB, 3.8 TB/s; the loads and maxima alone take 26).  Small: the
 // latency of the two phases (1 x 4 x 32000 float32: 10 us).
 // Exponentials are 32-bit, eight of them are added in 32 bits and from there on in 64; scores are 64-bit and rounded
 // once, so that the order of two candidates of one row is exact, and of different rows hangs on the logs of their rows'
-// sums alone.  These are within (3 ln n + 5) 2^-24 for n tokens; measured, 0.1e-8 to 2e-8 for rows of normal
-// logits (standard deviation 1 to 4, 32000 and 131072 tokens), and 2.5e-7 where all terms but the first are the same one.
+// sums alone.  These are within (3 ln n + 5) 2^-24 for n tokens; measured, 0.1e-8 to 2e-8 on average and 6e-8 at most for
+// rows of normal logits (standard deviation 1 to 4, 32000 and 131072 tokens), 2.5e-7 where all terms but the first are alike.
 struct SliceInfo {
     double sum;  // of exp(x - max)
     float max;
@@ -256,7 +256,7 @@ struct SliceInfo {
 };
 
 // Counters are lines of their own: slices of other items that count in the same line cost more than all of an item's
-// (4 x 4 x 131072: 12.2 us a call with one line for all, 10.3 so).
+// (4 x 4 x 131072: 12.2 us a call with one line for all, 10.5 so).
 constexpr uint32_t kCounterWords = 32;
 
 struct SelectArgs {
@@ -627,7 +627,7 @@ struct TilePart {
             const uint32_t from = at + j * 64 * V;
             raw[j] = Vec<T>::tail(x, 0);
             if (full || from + V <= vocab) {
-                // read once: nontemporal (64 x 8 x 131072, logits not in any cache: 40 -> 39 us)
+                // read once: nontemporal (64 x 8 x 131072, logits not in any cache: 37 -> 35 us)
                 typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(1)));
                 const Words w = __builtin_nontemporal_load(reinterpret_cast<const Words*>(x + from));
                 raw[j] = uint4{w.x, w.y, w.z, w.w};
@@ -685,8 +685,8 @@ __device__ __forceinline__ uint32_t larger(const uint64_t (*lists)[kWaveList + 8
 // one that k of its 1024 vectors' maxima reach (few more do, by their counts), then the k-th best of that
 // tile, in long slices later on one by the counts of all candidates.  Every wave collects its own in a list, so
 // nothing waits inside the loop over the other tiles.  The few vectors that hold a candidate go through a queue, where a
-// wave tests 64 of their elements at a time: a test and a branch for every element of a tile took 15 of 40 us
-// (64 x 8 x 131072 bfloat16, k = 16).
+// wave tests 64 of their elements at a time: a test and a branch for every element of a tile took 15 us
+// of a call's (64 x 8 x 131072 bfloat16, k = 16).
 // JOINED: the workgroup that finishes an item's last slice joins them.
 template <typename T, bool MASKED, bool JOINED>
 __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
@@ -732,8 +732,8 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
     const uint32_t mine = wave * (kTile / kWaves) + lane * V;
 
     // candidates are counted by their distance below the first tile's maximum, so that the threshold rises with the
-    // tiles: after n of them a tile has k / n candidates, not k (64 x 8 x 131072 bfloat16, a call: k = 16 36.7 -> 33.3 us,
-    // k = 64 50.5 -> 41.0).  Not in slices of few tiles (64 x 4 x 65536 float32, four tiles: 20.1 -> 20.9).
+    // tiles: after n of them a tile has k / n candidates, not k (64 x 8 x 131072 bfloat16, a call: k = 16 38 -> 35 us,
+    // k = 64 52 -> 42).  Not in slices of few tiles (64 x 4 x 65536 float32, four tiles: 20.6 -> 21.2).
     const bool counted = last - first > 4 * kTile;
     uint64_t* list = lists[wave];
     uint4* queue = lds.slice.queue[wave];
@@ -814,7 +814,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
         // sum of exponentials relative to the maximum, as powers of two.  log2 e is in two parts: the rounded factor alone is
         // 1.3e-8 off, always to the same side, which moves the logarithm of the sum by that times the mean distance from the
         // maximum (for a leader over a flat row of 2^24 the sum's log was 1.66e-7 off, with both parts it is 4e-9; 64 x 8 x 131072
-        // bfloat16, k = 16: 33.2 -> 34.7 us a call)
+        // bfloat16, k = 16: 33.2 -> 34.9 us a call)
         if (__any(most > ref)) {
             const float new_ref = wave_max(most);
             sum *= exp(static_cast<double>(ref) - static_cast<double>(new_ref));
@@ -844,7 +844,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(SelectArgs a) {
             }
             if (passing > k + 32) {
                 // a tile that is better than all before it: k of its own vectors set the threshold (a row that rises
-                // with the token, 64 x 8 x 131072: 720 us without this, 150 with it)
+                // with the token, 64 x 8 x 131072: 730 us without this, 158 with it)
                 uint32_t o[kVecs];
 #pragma unroll
                 for (int j = 0; j < kVecs; ++j) o[j] = ordered(top[j]);
@@ -1247,15 +1247,15 @@ namespace {
 
 // Slices that the rows of a call are cut into: the workgroups that 256 CUs hold at once.  With more, every slice's first
 // threshold and last ranking weigh more, and so does the join; with fewer, CUs have too little in flight (64 x 8 x
-// 131072, a call: 33 us at 1024 slices, 40 at 768, 39 at 1536, 40 at 2048).
+// 131072, a call: 35 us at 1024 slices, 37 at 512, 42 at 768, 41 at 1536 and 2048).
 constexpr uint64_t kSlicesWanted = 1024;
 
 // Calls within these limits are one launch: the last slice of an item joins its item.  Measured, a call as one launch
-// against two (bfloat16): 1 x 8 x 65536, k = 4: 9.6 against 10.1 us; 16 x 8 x 65536, k = 16: 14.2, 15.4; 500 x 2 x 32000: 21.9,
-// 25.4; 64 x 8 x 131072, k = 16: 35, 36.5.  Not more slices an item, which all count in one word (1 x 12 x 131072,
-// 192 of them: 11.6, 10.6; 1024: 32, 18), nor more entries or places than the join's 256 threads (the other join has
-// 1024) are quick with (1 x 2 x 131072, k = 128: 21.5, 17.4), nor more slices in all than the CUs hold at once (2000 x 8 x
-// 32000: 248, 215).
+// against two (bfloat16): 1 x 8 x 65536, k = 4: 9.9 against 10.2 us; 16 x 8 x 65536, k = 16: 14.2, 14.8; 500 x 2 x 32000,
+// k = 8: 23.5, 27.1; 64 x 8 x 131072, k = 16: 35, 35.5.  Not more slices an item, which all count in one word (1 x 12 x
+// 131072, k = 8, 192 of them: 12.5, 11.2; 1 x 64 x 131072, 1024 of them: 31, 17), nor more entries or places than the join's 256
+// threads (the other join has 1024) are quick with (1 x 2 x 131072, k = 128: 22, 17.4), nor more slices in all than the CUs
+// hold at once (2000 x 8 x 32000, k = 8: 260, 227).
 constexpr uint32_t kJoinedLists = 128, kJoinedEntries = 4096, kJoinedK = 64;
 
 struct Cut {
