@@ -86,3 +86,39 @@ def test_backtrace_of_the_most_steps(device, ends):
     for j in range(2):
         assert np.array_equal(got[0, j, :last], tokens[np.arange(last), 0, behind ^ j])
         assert (got[0, j, last:] == -1).all()
+
+
+def test_captured_reorder_and_backtrace(device):
+    """More states than one launch takes, with lengths, and the sequences with and without an output of the caller's, replayed
+    with other inputs and eager work in between."""
+    import torch
+    import radx_amd
+    batch, beams, total = 3, 4, 50
+    g = torch.Generator(device=device).manual_seed(5)
+    make = [lambda i=i: torch.randn(batch * beams, 2, 9 + i % 5, 8, generator=g, device=device) for i in range(30)]
+    states, eager = [m() for m in make], None
+    parents = torch.zeros(batch, beams, dtype=torch.int32, device=device)
+    lengths = torch.zeros(batch, dtype=torch.int32, device=device)
+    tokens, ways = (torch.zeros(total, batch, beams, dtype=torch.int32, device=device) for _ in range(2))
+    steps = torch.zeros(batch, dtype=torch.int32, device=device)
+    record = torch.full((batch, beams, total), -5, dtype=torch.int32, device=device)
+
+    def calls(states, record):
+        radx_amd.beam_reorder(states, parents, lengths=lengths, length_dim=2)
+        return radx_amd.beam_backtrace(tokens, ways, steps=steps), radx_amd.beam_backtrace(tokens, ways, steps=steps, out=record)
+
+    calls([s.clone() for s in states], record.clone())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        made, _ = calls(states, record)
+    for _ in range(4):
+        for t, low, high in ((parents, -1, beams + 1), (lengths, -1, 15), (tokens, 0, 1000), (ways, -1, beams + 1), (steps, -1, total + 3)):
+            t.copy_(torch.randint(low, high, t.shape, generator=g, device=device, dtype=torch.int32))
+        eager, again = [s.clone() for s in states], record.clone()
+        want, _ = calls(eager, again)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(s, e) for s, e in zip(states, eager))
+        assert torch.equal(made, want) and torch.equal(record, again)
+        torch.ones(100000, device=device).sum().item()
