@@ -284,7 +284,8 @@ size_t radx_hip_beam_scratch_bytes(uint32_t max_batch, uint32_t max_beams, uint3
  * (1..2^24) tokens, max_k (1..128) places, on HIP device `device`.  It owns the scratch of the call in flight: one
  * selection may be in flight per handle, also between two captured graphs, which it has to outlive.  Calls on several
  * streams have to be put in order by the caller, or be given a handle each: selections that overlap on one handle get wrong
- * results, and leave its counters so that later ones may, all without an error; such a handle is to be made anew.
+ * results, without an error.  Later ones do not, unless replayed graphs were among them or more than 16 in flight: such a
+ * handle is to be made anew.
  */
 int radx_hip_beam_create(int device, uint32_t max_batch, uint32_t max_beams, uint32_t max_vocab, uint32_t max_k,
                          radx_hip_beam** out);

@@ -72,7 +72,7 @@ def _plain(t, dtypes, shape, name, index):
 class BeamSelector:
     """One radx_hip_beam handle: the scratch of selections within these limits.  One selection may be in
     flight per handle; use one handle per concurrent stream or graph, or put the calls in order.  Selections that overlap on a
-    handle get wrong results, and later ones on it may, without an error; it has to outlive the graphs that captured it."""
+    handle get wrong results, without an error; it has to outlive the graphs that captured it."""
 
     def __init__(self, max_batch, max_beams, max_vocab, max_k, device=0):
         self.device = device

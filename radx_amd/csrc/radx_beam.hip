@@ -538,8 +538,9 @@ __device__ __forceinline__ void merge_item(const SelectArgs& a, uint32_t item, M
         a.scores[at] = score;
         a.parents[at] = parent;
         a.tokens[at] = token;
+        // (lists that calls overlapping by mistake have mixed may hold an entry twice, and a place no parent of the item)
         if (a.out_finished)
-            a.out_finished[at] = parent >= 0 && (token == a.end_token || a.finished[item * a.beams + parent]);
+            a.out_finished[at] = parent >= 0 && (token == a.end_token || a.finished[item * a.beams + min(static_cast<uint32_t>(parent), a.beams - 1u)]);
     }
 }
 
@@ -1241,6 +1242,7 @@ struct radx_hip_beam {
     int device = 0;
     uint32_t max_batch = 0, max_beams = 0, max_vocab = 0, max_k = 0;
     char* scratch = nullptr;
+    uint32_t calls = 0;  // made so far: the next one's counters
 };
 
 namespace {
@@ -1274,10 +1276,13 @@ uint64_t most_slices(uint64_t rows, uint64_t vocab) {
     const uint64_t all = rows * tiles;
     return all < kSlicesWanted + rows ? all : kSlicesWanted + rows;
 }
-// Counters for the items of calls that are one launch: such a call has kSlicesWanted slices at most.
+// Counters for the items of calls that are one launch: such a call has kSlicesWanted slices at most.  A handle's calls take
+// its sets of counters in turn, so that two which overlap by mistake, and spoil each other's lists, leave none behind that
+// has counted slices of both: every later call would join too early, or never.
+constexpr uint32_t kCounterSets = 16;
 uint64_t arrived_bytes(uint64_t batch) { return (batch < kSlicesWanted ? batch : kSlicesWanted) * kCounterWords * 4; }
 uint64_t scratch_of(uint64_t batch, uint64_t beams, uint64_t vocab, uint64_t k) {
-    return arrived_bytes(batch) + most_slices(batch * beams, vocab) * (sizeof(SliceInfo) + k * 8);
+    return kCounterSets * arrived_bytes(batch) + most_slices(batch * beams, vocab) * (sizeof(SliceInfo) + k * 8);
 }
 
 uint32_t inverse(uint32_t d) { return static_cast<uint32_t>((0xffffffffull + d) / d); }  // ceil(2^32 / d)
@@ -1364,7 +1369,7 @@ int radx_hip_beam_create(int device, uint32_t max_batch, uint32_t max_beams, uin
     h->max_k = max_k;
     const hipError_t e = hipMalloc(reinterpret_cast<void**>(&h->scratch), radx_hip_beam_scratch_bytes(max_batch, max_beams, max_vocab, max_k));
     if (e != hipSuccess) { delete h; return fail(e, "hipMalloc(scratch)"); }
-    hipError_t z = hipMemset(h->scratch, 0, arrived_bytes(max_batch));
+    hipError_t z = hipMemset(h->scratch, 0, kCounterSets * arrived_bytes(max_batch));
     if (z == hipSuccess) z = hipStreamSynchronize(nullptr);  // other streams do not wait for the null stream
     if (z != hipSuccess) { (void)hipFree(h->scratch); delete h; return fail(z, "hipMemset(scratch)"); }
     *out = h;
@@ -1431,8 +1436,8 @@ int radx_hip_beam_select(radx_hip_beam* h, const radx_hip_beam_select_args* s, v
     a.tiles_per_slice = cut.tiles_per_slice;
     a.k_inverse = inverse(a.k);
     a.slices_inverse = inverse(a.slices);
-    a.arrived = reinterpret_cast<uint32_t*>(h->scratch);
-    char* const slices = h->scratch + arrived_bytes(h->max_batch);
+    a.arrived = reinterpret_cast<uint32_t*>(h->scratch + h->calls++ % kCounterSets * arrived_bytes(h->max_batch));
+    char* const slices = h->scratch + kCounterSets * arrived_bytes(h->max_batch);
     a.info = reinterpret_cast<SliceInfo*>(slices);
     a.best = reinterpret_cast<uint64_t*>(slices + most_slices(static_cast<uint64_t>(h->max_batch) * h->max_beams, h->max_vocab) * sizeof(SliceInfo));
     a.scores = s->scores;

@@ -122,3 +122,39 @@ def test_captured_reorder_and_backtrace(device):
         assert all(torch.equal(s, e) for s, e in zip(states, eager))
         assert torch.equal(made, want) and torch.equal(record, again)
         torch.ones(100000, device=device).sum().item()
+
+
+def test_calls_that_overlapped_leave_the_handle_as_it_was(device):
+    """Two selections of one handle on two streams, in no order: their results are nobody's, as documented, but later calls are
+    right again, whichever of the handle's counters they take."""
+    import torch
+    import radx_amd
+    from test_gpu_beam import check_best, make_logits, plain_scores, run_select
+    sel = radx_amd.BeamSelector(8, 4, 131072, 8)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    calls = []
+    for batch, beams, vocab, k, dtype in ((4, 4, 131072, 8, "bf16"), (8, 4, 32000, 8, "bf16")):
+        logits, x = make_logits(batch, beams, vocab, dtype, device, seed=vocab)
+        cum = (-np.random.default_rng(k).random((batch, beams))).astype(np.float32)
+        calls.append((logits, x, cum, on(cum, device), k))
+    torch.cuda.synchronize()
+    outs = [sel.select(logits, dev_cum, k) for logits, _, _, dev_cum, k in calls]
+    work = torch.zeros(1 << 26, device=device)
+    for _ in range(25):
+        for _ in range(4):
+            work.add_(1.0)  # both streams wait for this, so that their calls start together
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        for _ in range(3):  # fewer in flight than the handle has sets of counters
+            for s, (logits, _, _, dev_cum, k), out in zip(streams, calls, outs):
+                sel.select(logits, dev_cum, k, out=out, stream=s)
+        torch.cuda.synchronize()
+    want = []
+    for turn in range(40):
+        logits, x, cum, dev_cum, k = calls[turn % 2]
+        got = run_select(sel, logits, dev_cum, k)
+        if turn < 2:
+            check_best(got, plain_scores(x, cum), x, k, x.shape[2])
+            want.append(got)
+        assert all(np.array_equal(g, w) for g, w in zip(got, want[turn % 2])), turn
+    sel.close()
